@@ -35,9 +35,28 @@ class Rope(C.Structure):
                 ("n_rdim", C.c_int32), ("max_h", C.c_int32), ("max_w", C.c_int32)]
 
 
+class RopeAxes(C.Structure):
+    _fields_ = [("pos", C.c_void_p), ("pos_stride", C.c_int64 * 2), ("n_axes", C.c_int32), ("n_pairs", C.c_int32 * 4),
+                ("max_pos", C.c_int32 * 4), ("cs", C.c_void_p * 4)]
+
+
+class SinkGeom(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("B", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("N", C.c_int32), ("d_qk", C.c_int32),
+                ("d_v", C.c_int32), ("window", C.c_int32), ("n_sink", C.c_int32), ("sm_scale", C.c_float), ("impl", C.c_int32),
+                ("lens", C.c_void_p)]
+
+
+class SinkCache(C.Structure):
+    _fields_ = [("k", Tensor4), ("v", Tensor4), ("page_table", C.c_void_p), ("seq_lens", C.c_void_p), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32), ("max_pages", C.c_int32)]
+
+
 EXPORTS = ("swa_fwd", "swa_bwd_delta", "swa_bwd_dq", "swa_bwd_dkdv", "swa_fwd_rot", "swa_bwd_dq_rot", "swa_bwd_dkdv_rot",
            "swa_bwd_noalloc", "swa_step_select", "swa_step_select_impl", "swa_step_describe_plan", "swa_step_fwd", "swa_step_bwd",
            "rope2d_apply", "rope2d_apply_to", "swa_select_impl", "swa_describe_plan", "swa_refresh_env", "swa_launch_count", "swa_last_error", "swa_version")
+# ... and of include/swa_sequence.h
+SEQUENCE_EXPORTS = ("rope_axes_apply", "sink_swa_select", "sink_swa_fwd", "sink_swa_bwd_scratch", "sink_swa_bwd", "kv_append_rope",
+                    "sink_swa_decode")
 
 
 def _load() -> C.CDLL:
@@ -73,6 +92,17 @@ def _load() -> C.CDLL:
                                  C.c_void_p, P(Tensor4), P(Tensor4), P(Tensor4), C.c_void_p, C.c_void_p]
     lib.swa_select_impl.argtypes = [P(Geom), P(Rope), C.c_int32]
     lib.swa_describe_plan.argtypes = [P(Geom), P(Rope), C.c_int32, P(C.c_int32)]
+    T, i32, ptr = P(Tensor4), C.c_int32, C.c_void_p
+    lib.rope_axes_apply.argtypes = [i32, P(RopeAxes), i32, C.c_int64, i32, T, T, i32, T, T, i32, i32, ptr]
+    lib.sink_swa_select.argtypes = [P(SinkGeom)]
+    lib.sink_swa_fwd.argtypes = [P(SinkGeom), T, T, T, T, ptr, ptr, ptr]
+    lib.sink_swa_bwd_scratch.argtypes = [P(SinkGeom)]
+    lib.sink_swa_bwd_scratch.restype = C.c_int64
+    lib.sink_swa_bwd.argtypes = [P(SinkGeom), T, T, T, T, T, ptr, T, T, T, ptr, C.c_int64, ptr, ptr]
+    lib.kv_append_rope.argtypes = [i32, P(RopeAxes), i32, i32, i32, i32, i32, i32, T, T, T, T, P(SinkCache), ptr, ptr]
+    lib.sink_swa_decode.argtypes = [i32] * 8 + [C.c_float, i32, T, P(SinkCache), T, ptr]
+    for name in ("rope_axes_apply", "sink_swa_select", "sink_swa_fwd", "sink_swa_bwd", "kv_append_rope", "sink_swa_decode"):
+        getattr(lib, name).restype = C.c_int
     for name in ("swa_fwd", "swa_bwd_delta", "swa_bwd_dq", "swa_bwd_dkdv", "swa_fwd_rot", "swa_bwd_dq_rot",
                  "swa_bwd_dkdv_rot", "swa_bwd_noalloc", "swa_step_select", "swa_step_select_impl", "swa_step_describe_plan", "swa_step_fwd",
                  "swa_step_bwd", "rope2d_apply",

@@ -20,7 +20,7 @@ EXT = os.path.join(HERE, "_swa2d_torch.so")
 # source -> extra flags.  The tensor-core kernels are built with fast math (ex2.approx / ftz in their softmax loops:
 # their outputs are 16-bit); the C ABI file holds the SIMT kernels, whose fp32 path must hold 1e-4 against the
 # oracle, and is built with IEEE division and exp2.
-SOURCES = {"swa_abi.cu": [], "swa_tc.cu": ["--use_fast_math"]}
+SOURCES = {"swa_abi.cu": [], "swa_tc.cu": ["--use_fast_math"], "sink_abi.cu": [], "sink_tc.cu": ["--use_fast_math"]}
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
 
 
@@ -48,7 +48,7 @@ def needs_build() -> bool:
     if not os.path.exists(LIB) or not os.path.exists(EXT):
         return True
     t = min(os.path.getmtime(LIB), os.path.getmtime(EXT))
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", "swa2d.h")]
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", h) for h in ("swa2d.h", "swa_sequence.h")]
     return any(os.path.getmtime(d) > t for d in deps if os.path.isfile(d))
 
 

@@ -1,0 +1,357 @@
+// C ABI (include/swa2d.h) of the operators for token sequences: argument validation, kernel-family selection, launches.
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+
+#include "common.cuh"
+#include "rope_axes.cuh"
+#include "sink_decode.cuh"
+#include "sink_rows.cuh"
+#include "sink_tc.cuh"
+
+namespace swa {
+int abi_fail(int code, const char* msg);
+int abi_launched(const char* what);
+}  // namespace swa
+
+namespace {
+
+using swa::abi_launched;
+
+enum : int { E_NULL = -1, E_DTYPE = -2, E_SHAPE = -3, E_ROPE = -4, E_IMPL = -5, E_LAUNCH = -6, E_STRIDE = -7 };
+
+int fail(int code, const char* fmt, ...) {
+  char msg[400];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(msg, sizeof(msg), fmt, ap);
+  va_end(ap);
+  return swa::abi_fail(code, msg);
+}
+
+int check_tensor(const swa_tensor_t* t, const char* name) {
+  if (!t || !t->ptr) return fail(E_NULL, "%s is NULL", name);
+  return 0;
+}
+int check_dtype(int32_t dtype) {
+  if (dtype < SWA_F32 || dtype > SWA_BF16) return fail(E_DTYPE, "unknown dtype %d", dtype);
+  return 0;
+}
+
+int check_axes(const rope_axes_t* r, int32_t C) {
+  if (!r) return fail(E_NULL, "rope axes are NULL");
+  if (r->n_axes < 1 || r->n_axes > ROPE_MAX_AXES) return fail(E_ROPE, "n_axes must be in [1, %d]", ROPE_MAX_AXES);
+  int64_t pairs = 0;
+  for (int a = 0; a < r->n_axes; ++a) {
+    if (r->n_pairs[a] <= 0 || r->max_pos[a] <= 0) return fail(E_ROPE, "axis %d: pairs and table rows must be positive", a);
+    if (!r->cs[a]) return fail(E_ROPE, "axis %d: table is NULL", a);
+    pairs += r->n_pairs[a];
+  }
+  if (2 * pairs > C) return fail(E_ROPE, "2 * pairs of all axes (%lld) exceeds the head dim %d", (long long)(2 * pairs), C);
+  return 0;
+}
+
+int check_heads(int32_t B, int32_t Hq, int32_t Hkv) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0) return fail(E_SHAPE, "batch and heads must be positive");
+  if (Hq % Hkv) return fail(E_SHAPE, "query heads (%d) must be a multiple of key heads (%d)", Hq, Hkv);
+  if (B > 65535 || Hq > 65535) return fail(E_SHAPE, "batch and heads must be at most 65535");
+  return 0;
+}
+
+int check_geom(const sink_geom_t* g) {
+  if (!g) return fail(E_NULL, "geometry is NULL");
+  if (int e = check_dtype(g->dtype)) return e;
+  if (int e = check_heads(g->B, g->Hq, g->Hkv)) return e;
+  if (g->N <= 0 || g->N > (1 << 30)) return fail(E_SHAPE, "tokens must be in [1, 2^30]");
+  if (g->d_qk <= 0 || g->d_v <= 0 || g->d_qk > swa::sink::kMaxDim || g->d_v > swa::sink::kMaxDim)
+    return fail(E_SHAPE, "head dims must be in [1, %d]", swa::sink::kMaxDim);
+  if (g->window < 1) return fail(E_SHAPE, "window must be at least 1 (a token sees itself)");
+  if (g->n_sink < 0 || g->n_sink > SINK_MAX_SINKS) return fail(E_SHAPE, "n_sink must be in [0, %d]", SINK_MAX_SINKS);
+  if (g->impl < SWA_IMPL_AUTO || g->impl > SWA_IMPL_TC) return fail(E_IMPL, "unknown impl %d", g->impl);
+  return 0;
+}
+
+swa::sink::Args make_args(const sink_geom_t* g) {
+  swa::sink::Args a;
+  memset(&a, 0, sizeof(a));
+  a.lens = g->lens;
+  a.B = g->B; a.Hq = g->Hq; a.Hkv = g->Hkv; a.G = g->Hq / g->Hkv; a.N = g->N;
+  a.dqk = g->d_qk; a.dv_dim = g->d_v;
+  a.W = std::min(g->window, g->N);
+  a.ns = std::min(g->n_sink, g->N);
+  a.scale = g->sm_scale;
+  a.c2 = g->sm_scale * swa::kLog2e;
+  return a;
+}
+
+int resolve(const sink_geom_t* g, const swa_tensor_t* const* ts, int n) {
+  const char* why = swa::sink::tc_unsupported(g, ts, n);
+  if (g->impl == SWA_IMPL_SIMT) return SWA_IMPL_SIMT;
+  if (!why) return SWA_IMPL_TC;
+  if (g->impl == SWA_IMPL_TC) return fail(E_IMPL, "tensor-core path unavailable: %s", why);
+  return SWA_IMPL_SIMT;
+}
+
+#define SINK_DISPATCH(dtype, ...)                                 \
+  do {                                                            \
+    switch (dtype) {                                              \
+      case SWA_F32: { using T = float; __VA_ARGS__; break; }      \
+      case SWA_F16: { using T = __half; __VA_ARGS__; break; }     \
+      default: { using T = __nv_bfloat16; __VA_ARGS__; break; }   \
+    }                                                             \
+  } while (0)
+
+int launched(cudaError_t e, const char* what) {
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(E_LAUNCH, "%s launch failed: %s", what, cudaGetErrorString(e));
+  }
+  return abi_launched(what);
+}
+
+template <int KIND>
+int launch_rows(const swa::sink::Args& a, int dtype, cudaStream_t st) {
+  const dim3 grid((unsigned)((a.N + swa::sink::kRowWarps - 1) / swa::sink::kRowWarps), KIND == 2 ? a.Hkv : a.Hq, a.B);
+  cudaError_t e = cudaSuccess;
+  SINK_DISPATCH(dtype, e = swa::launch_pdl(swa::sink::rows_kernel<T, KIND>, grid, 32 * swa::sink::kRowWarps, 0, st, a));
+  return launched(e, KIND == 0 ? "sink rows forward" : KIND == 1 ? "sink rows dQ" : "sink rows dK/dV");
+}
+
+// ---- rotation --------------------------------------------------------------------------------------------------------
+bool aligned(const swa_tensor_t& t, int ve, int esz) {
+  if (ve == 1) return true;
+  return t.stride[3] == 1 && (uintptr_t)t.ptr % (ve * esz) == 0 && t.stride[0] % ve == 0 && t.stride[1] % ve == 0 && t.stride[2] % ve == 0;
+}
+
+// Launches the groups of `a` (g[i].H > 0) with the widest unit that all of them, the axes and the tables allow.
+int launch_rotate(swa::axes::Args& a, int n_groups, const swa_tensor_t* const* tensors, int n_tensors, int dtype, int B, cudaStream_t st) {
+  const int esz = dtype == SWA_F32 ? 4 : 2;
+  bool rotates = false;
+  for (int i = 0; i < n_groups; ++i) rotates |= a.g[i].rotate != 0;
+  auto fits = [&](int ve) {
+    for (int i = 0; i < n_groups; ++i)
+      if (a.g[i].d % ve) return false;
+    for (int i = 0; i < n_tensors; ++i)
+      if (!aligned(*tensors[i], ve, esz)) return false;
+    for (int x = 0; rotates && x < a.n_axes; ++x)
+      if (a.R[x] % ve || (ve > 1 && (uintptr_t)a.cs[x] % 16)) return false;
+    return true;
+  };
+  int ve = 16 / esz;
+  while (!fits(ve)) ve >>= 1;
+  int64_t spr = 0;
+  int heads = 0;
+  for (int i = 0; i < n_groups; ++i) {
+    const int64_t rot = a.g[i].rotate ? a.pairs / ve : 0;
+    spr = std::max(spr, rot + (a.g[i].d / ve - 2 * rot + 1) / 2);
+    heads += a.g[i].H;
+  }
+  if (a.N * spr > INT32_MAX) return fail(E_SHAPE, "too many tokens in one call");
+  const int64_t blocks = (a.N * spr + 255) / 256;
+  // Four heads a thread where that leaves two blocks for every place on the SMs (8 of 148): their loads are in flight together and the
+  // table is read once.
+  const bool four = blocks * B * ((heads + 3) / 4) >= 2 * 8 * 148;
+  unsigned chunks = 0;
+  for (int i = 0; i < n_groups; ++i) chunks += a.g[i].chunks = four ? (a.g[i].H + 3) / 4 : a.g[i].H;
+  if (chunks > 65535) return fail(E_SHAPE, "too many heads");
+  const dim3 grid((unsigned)blocks, chunks, B);
+  cudaError_t e = cudaSuccess;
+#define ROT(T, VE) e = four ? swa::launch_stream(swa::axes::rotate_kernel<T, VE, 4>, grid, 256, st, a) : swa::launch_stream(swa::axes::rotate_kernel<T, VE, 1>, grid, 256, st, a)
+#define ROT16(T) do { if (ve == 8) ROT(T, 8); else if (ve == 4) ROT(T, 4); else if (ve == 2) ROT(T, 2); else ROT(T, 1); } while (0)
+  if (dtype == SWA_F32) {
+    if (ve == 4) ROT(float, 4); else if (ve == 2) ROT(float, 2); else ROT(float, 1);
+  } else if (dtype == SWA_F16) {
+    ROT16(__half);
+  } else {
+    ROT16(__nv_bfloat16);
+  }
+#undef ROT16
+#undef ROT
+  return launched(e, "rotate");
+}
+
+void set_axes(swa::axes::Args* a, const rope_axes_t* r) {
+  a->n_axes = r->n_axes;
+  a->pairs = 0;
+  for (int x = 0; x < r->n_axes; ++x) {
+    a->R[x] = r->n_pairs[x];
+    a->max_pos[x] = r->max_pos[x];
+    a->cs[x] = r->cs[x];
+    a->pairs += r->n_pairs[x];
+  }
+  a->pos = r->pos;
+  a->pos_b = r->pos_stride[0];
+  a->pos_a = r->pos_stride[1];
+}
+
+int check_cache(const sink_cache_t* c) {
+  if (!c) return fail(E_NULL, "cache is NULL");
+  if (int e = check_tensor(&c->k, "k cache")) return e;
+  if (int e = check_tensor(&c->v, "v cache")) return e;
+  if (!c->page_table || !c->seq_lens) return fail(E_NULL, "page_table or seq_lens is NULL");
+  if (c->n_pages <= 0 || c->page_size <= 0 || c->max_pages <= 0) return fail(E_SHAPE, "pages, page size and table width must be positive");
+  if ((int64_t)c->max_pages * c->page_size > (1 << 30)) return fail(E_SHAPE, "a sequence may hold at most 2^30 tokens");
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rope_axes_apply(int32_t dtype, const rope_axes_t* r, int32_t B, int64_t N, int32_t C, const swa_tensor_t* x, const swa_tensor_t* y,
+                    int32_t H, const swa_tensor_t* x2, const swa_tensor_t* y2, int32_t H2, int32_t inverse, void* stream) {
+  if (int e = check_dtype(dtype)) return e;
+  if (B <= 0 || B > 65535 || N <= 0 || N > INT32_MAX || C <= 0 || H <= 0 || (x2 && H2 <= 0)) return fail(E_SHAPE, "bad batch, tokens, heads or head dim");
+  if (int e = check_axes(r, C)) return e;
+  if (!r->pos) return fail(E_NULL, "positions are NULL");
+  if (int e = check_tensor(x, "x")) return e;
+  if (int e = check_tensor(y, "y")) return e;
+  if (x2) {
+    if (int e = check_tensor(x2, "x2")) return e;
+    if (int e = check_tensor(y2, "y2")) return e;
+  }
+  swa::axes::Args a;
+  memset(&a, 0, sizeof(a));
+  set_axes(&a, r);
+  a.N = (int)N;
+  a.sign = inverse ? -1.f : 1.f;
+  a.g[0] = swa::axes::Group{swa::make_view(x), swa::make_view(y), H, C, 1, 0, 0};
+  if (x2) a.g[1] = swa::axes::Group{swa::make_view(x2), swa::make_view(y2), H2, C, 1, 0, 0};
+  const swa_tensor_t* ts[] = {x, y, x2, y2};
+  return launch_rotate(a, x2 ? 2 : 1, ts, x2 ? 4 : 2, dtype, B, (cudaStream_t)stream);
+}
+
+int kv_append_rope(int32_t dtype, const rope_axes_t* r, int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t d_qk, int32_t d_v,
+                   const swa_tensor_t* q, const swa_tensor_t* q_out, const swa_tensor_t* k, const swa_tensor_t* v,
+                   const sink_cache_t* cache, const int32_t* new_lens, void* stream) {
+  if (int e = check_dtype(dtype)) return e;
+  if (B <= 0 || B > 65535 || Hkv <= 0 || T <= 0 || d_qk <= 0 || d_v <= 0 || (q && Hq <= 0)) return fail(E_SHAPE, "bad batch, tokens, heads or head dim");
+  const bool rot = r && r->pos;
+  if (rot)
+    if (int e = check_axes(r, d_qk)) return e;
+  if (int e = check_tensor(k, "k")) return e;
+  if (int e = check_tensor(v, "v")) return e;
+  if (int e = check_cache(cache)) return e;
+  if ((q != nullptr) != (q_out != nullptr)) return fail(E_NULL, "q and q_out go together");
+  if (q) {
+    if (int e = check_tensor(q, "q")) return e;
+    if (int e = check_tensor(q_out, "q_out")) return e;
+  }
+  swa::axes::Args a;
+  memset(&a, 0, sizeof(a));
+  if (rot) set_axes(&a, r);
+  a.N = T;
+  a.sign = 1.f;
+  a.page_table = cache->page_table;
+  a.seq_lens = cache->seq_lens;
+  a.new_lens = new_lens;
+  a.max_pages = cache->max_pages;
+  a.n_pages = cache->n_pages;
+  a.page_size = cache->page_size;
+  const swa_tensor_t* ts[6] = {k, &cache->k, v, &cache->v, q, q_out};
+  a.g[0] = swa::axes::Group{swa::make_view(k), swa::make_view(&cache->k), Hkv, d_qk, rot, 1, 0};
+  a.g[1] = swa::axes::Group{swa::make_view(v), swa::make_view(&cache->v), Hkv, d_v, 0, 1, 0};
+  if (q) a.g[2] = swa::axes::Group{swa::make_view(q), swa::make_view(q_out), Hq, d_qk, rot, 0, 0};
+  return launch_rotate(a, q ? 3 : 2, ts, q ? 6 : 4, dtype, B, (cudaStream_t)stream);
+}
+
+int sink_swa_select(const sink_geom_t* g) {
+  if (int e = check_geom(g)) return e;
+  return resolve(g, nullptr, 0);
+}
+
+int sink_swa_fwd(const sink_geom_t* g, const swa_tensor_t* q, const swa_tensor_t* k, const swa_tensor_t* v, const swa_tensor_t* o,
+                 float* lse, int32_t* status, void* stream) {
+  if (int e = check_geom(g)) return e;
+  if (int e = check_tensor(q, "q")) return e;
+  if (int e = check_tensor(k, "k")) return e;
+  if (int e = check_tensor(v, "v")) return e;
+  if (int e = check_tensor(o, "o")) return e;
+  if (!lse) return fail(E_NULL, "lse is NULL");
+  const swa_tensor_t* ts[] = {q, k, v, o};
+  const int impl = resolve(g, ts, 4);
+  if (impl < 0) return impl;
+  cudaStream_t st = (cudaStream_t)stream;
+  swa::sink::Args a = make_args(g);
+  a.q = swa::make_view(q); a.k = swa::make_view(k); a.v = swa::make_view(v); a.o = swa::make_view(o);
+  a.lse = lse;
+  if (impl == SWA_IMPL_TC) {
+    if (swa::sink::tc_fwd(a, g->dtype, status, st)) return fail(E_LAUNCH, "tcgen05 sink forward: %s", swa::sink::tc_error());
+    return abi_launched("tcgen05 sink forward");
+  }
+  return launch_rows<0>(a, g->dtype, st);
+}
+
+static int64_t delta_bytes(const sink_geom_t* g) { return ((int64_t)g->B * g->Hq * g->N * 4 + 255) / 256 * 256; }
+
+int64_t sink_swa_bwd_scratch(const sink_geom_t* g) {
+  if (int e = check_geom(g)) return e;
+  const int impl = resolve(g, nullptr, 0);
+  if (impl < 0) return impl;
+  return delta_bytes(g) + (impl == SWA_IMPL_TC ? swa::sink::tc_bwd_scratch(make_args(g)) : 0);
+}
+
+int sink_swa_bwd(const sink_geom_t* g, const swa_tensor_t* q, const swa_tensor_t* k, const swa_tensor_t* v, const swa_tensor_t* o,
+                 const swa_tensor_t* d_o, const float* lse, const swa_tensor_t* dq, const swa_tensor_t* dk, const swa_tensor_t* dv,
+                 void* scratch, int64_t scratch_bytes, int32_t* status, void* stream) {
+  if (int e = check_geom(g)) return e;
+  const swa_tensor_t* ts[] = {q, k, v, o, d_o, dq, dk, dv};
+  const char* names[] = {"q", "k", "v", "o", "do", "dq", "dk", "dv"};
+  for (int i = 0; i < 8; ++i)
+    if (int e = check_tensor(ts[i], names[i])) return e;
+  if (!lse || !scratch) return fail(E_NULL, "lse or scratch is NULL");
+  const int impl = resolve(g, ts, 8);
+  if (impl < 0) return impl;
+  const int64_t need = delta_bytes(g) + (impl == SWA_IMPL_TC ? swa::sink::tc_bwd_scratch(make_args(g)) : 0);
+  if (scratch_bytes < need || (uintptr_t)scratch % 16) return fail(E_SHAPE, "scratch: %lld bytes on a 16-byte boundary needed", (long long)need);
+  cudaStream_t st = (cudaStream_t)stream;
+  swa::sink::Args a = make_args(g);
+  a.q = swa::make_view(q); a.k = swa::make_view(k); a.v = swa::make_view(v); a.o = swa::make_view(o); a.d_o = swa::make_view(d_o);
+  a.dq = swa::make_view(dq); a.dk = swa::make_view(dk); a.dv = swa::make_view(dv);
+  a.lse = const_cast<float*>(lse);
+  a.delta = (float*)scratch;
+  swa_geom_t sg;
+  memset(&sg, 0, sizeof(sg));
+  sg.dtype = g->dtype; sg.B = g->B; sg.H = g->Hq; sg.b_size = 1; sg.t_height = g->N; sg.t_width = 1; sg.d_qk = g->d_qk; sg.d_v = g->d_v;
+  sg.sm_scale = g->sm_scale;
+  if ((int64_t)g->B * g->Hq > 65535) return fail(E_SHAPE, "B*Hq exceeds 65535");
+  if (int e = swa_bwd_delta(&sg, o, d_o, a.delta, stream)) return e;
+  if (impl == SWA_IMPL_TC) {
+    int launches = 0;
+    if (swa::sink::tc_bwd(a, g->dtype, (char*)scratch + delta_bytes(g), status, st, &launches))
+      return fail(E_LAUNCH, "tcgen05 sink backward: %s", swa::sink::tc_error());
+    for (int i = 0; i < launches; ++i)
+      if (int e = abi_launched("tcgen05 sink backward")) return e;
+    return 0;
+  }
+  if (int e = launch_rows<1>(a, g->dtype, st)) return e;
+  return launch_rows<2>(a, g->dtype, st);
+}
+
+int sink_swa_decode(int32_t dtype, int32_t B, int32_t Hq, int32_t Hkv, int32_t d_qk, int32_t d_v, int32_t window, int32_t n_sink,
+                    float sm_scale, int32_t impl, const swa_tensor_t* q, const sink_cache_t* cache, const swa_tensor_t* o, void* stream) {
+  if (int e = check_dtype(dtype)) return e;
+  if (int e = check_heads(B, Hq, Hkv)) return e;
+  if (d_qk <= 0 || d_v <= 0 || d_qk > swa::sink::kMaxDim || d_v > swa::sink::kMaxDim)
+    return fail(E_SHAPE, "head dims must be in [1, %d]", swa::sink::kMaxDim);
+  if (window < 1) return fail(E_SHAPE, "window must be at least 1 (a token sees itself)");
+  if (n_sink < 0 || n_sink > SINK_MAX_SINKS) return fail(E_SHAPE, "n_sink must be in [0, %d]", SINK_MAX_SINKS);
+  if (impl < SWA_IMPL_AUTO || impl > SWA_IMPL_TC) return fail(E_IMPL, "unknown impl %d", impl);
+  if (int e = check_tensor(q, "q")) return e;
+  if (int e = check_tensor(o, "o")) return e;
+  if (int e = check_cache(cache)) return e;
+  swa::sink::DecodeArgs a;
+  memset(&a, 0, sizeof(a));
+  a.q = swa::make_view(q); a.o = swa::make_view(o); a.k = swa::make_view(&cache->k); a.v = swa::make_view(&cache->v);
+  a.page_table = cache->page_table; a.seq_lens = cache->seq_lens;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.dqk = d_qk; a.dv = d_v; a.W = window; a.ns = n_sink;
+  a.max_pages = cache->max_pages; a.n_pages = cache->n_pages; a.page_size = cache->page_size;
+  a.c2 = sm_scale * swa::kLog2e;
+  const dim3 grid((Hq + swa::sink::kRowWarps - 1) / swa::sink::kRowWarps, B);
+  cudaError_t e = cudaSuccess;
+  SINK_DISPATCH(dtype, e = swa::launch_pdl(swa::sink::decode_rows_kernel<T>, grid, 32 * swa::sink::kRowWarps, 0, (cudaStream_t)stream, a));
+  return launched(e, "sink decode");
+}
+
+}  // extern "C"

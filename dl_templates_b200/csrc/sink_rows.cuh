@@ -1,0 +1,209 @@
+// Attention with a sliding window and sink tokens, one warp per row: token i of a sequence of `len` tokens sees token j if
+//   j <= i,  i < len  and  (j > i - W  or  j < n_sink).
+// These functions are the definition the tiled kernels are held to: only pairs that see each other are touched, so that an
+// infinity or a NaN stays with the rows that see it.  They serve every type, stride and head dim up to 256, and the tiled kernels
+// fall back on them for the rows (and only those) in which an infinity or a NaN has turned up: a hidden pair weighs 0 there, and
+// 0 * inf is a NaN.
+#pragma once
+
+#include "../../include/swa_sequence.h"
+#include "common.cuh"
+
+namespace swa {
+namespace sink {
+
+constexpr int kMaxDim = 256, kDimsPerLane = kMaxDim / 32;
+
+struct Args {
+  View4 q, k, v, o, d_o, dq, dk, dv;
+  float* lse;            // [B, Hq, N], base 2
+  float* delta;          // [B, Hq, N]: sum of o * do
+  const int32_t* lens;   // [B] or nullptr: all N
+  int B, Hq, Hkv, G, N, dqk, dv_dim, W, ns;
+  float scale, c2;       // c2 = scale * log2(e)
+};
+
+__device__ __forceinline__ int seq_len(const Args& a, int b) {
+  if (!a.lens) return a.N;
+  const int n = a.lens[b];
+  return n < 0 ? 0 : n > a.N ? a.N : n;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row_ptr(const View4& v, int b, int h, int n) {
+  return (const T*)v.ptr + b * v.s0 + h * v.s1 + (int64_t)n * v.s2;
+}
+
+template <typename T>
+__device__ __forceinline__ void stage_row(float* s, const T* p, int64_t st, int d, int lane) {
+  for (int t = lane; t < d; t += 32) s[t] = to_f(p[t * st]);
+}
+
+// s . row, the row read by one lane; by 16 bytes where the tensor allows.
+template <typename T>
+__device__ __forceinline__ float dot_row(const float* s, const T* p, int64_t st, int d, bool vec) {
+  float acc = 0.f;
+  if (vec) {
+    constexpr int E = 16 / sizeof(T);
+    for (int t = 0; t < d; t += E) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p + t);
+      const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int x = 0; x < E; ++x) acc = fmaf(s[t + x], to_f(e[x]), acc);
+    }
+  } else {
+    for (int t = 0; t < d; ++t) acc = fmaf(s[t], to_f(p[t * st]), acc);
+  }
+  return acc;
+}
+
+template <typename T>
+__device__ __forceinline__ bool vec_rows(const View4& v, int d) {
+  constexpr int E = 16 / sizeof(T);
+  return v.s3 == 1 && d % E == 0 && reinterpret_cast<uintptr_t>(v.ptr) % 16 == 0 && v.s0 % E == 0 && v.s1 % E == 0 && v.s2 % E == 0;
+}
+
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// acc += sum over the chunk's keys of w[key] * row[key]: each lane owns dims lane, lane + 32, ...; `see` has a bit per key.
+template <typename T>
+__device__ __forceinline__ void add_rows(float* acc, float w, uint32_t see, const T* base, int64_t s2, int64_t s3, int d, int lane) {
+  while (see) {
+    const int j = __ffs(see) - 1;
+    see &= see - 1;
+    const float x = __shfl_sync(0xffffffffu, w, j);
+    const T* p = base + j * s2;
+#pragma unroll
+    for (int t = 0; t < kDimsPerLane; ++t)
+      if (lane + 32 * t < d) acc[t] = fmaf(x, to_f(p[(lane + 32 * t) * s3]), acc[t]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_row(const View4& v, int b, int h, int n, const float* acc, float f, int d, int lane) {
+  T* p = (T*)v.ptr + b * v.s0 + h * v.s1 + (int64_t)n * v.s2;
+#pragma unroll
+  for (int t = 0; t < kDimsPerLane; ++t)
+    if (lane + 32 * t < d) p[(lane + 32 * t) * v.s3] = from_f<T>(acc[t] * f);
+}
+
+// Calls body(first key, bits of its 32 keys that row i sees) for every chunk with such a key.
+template <typename F>
+__device__ __forceinline__ void for_key_chunks(const Args& a, int i, int lane, F&& body) {
+  const int lo = max(0, i - a.W + 1), sinks = min(a.ns, lo);
+  for (int j0 = 0; j0 < sinks; j0 += 32) body(j0, __ballot_sync(0xffffffffu, j0 + lane < sinks));
+  for (int j0 = lo; j0 <= i; j0 += 32) body(j0, __ballot_sync(0xffffffffu, j0 + lane <= i));
+}
+
+// Forward: o_i and lse_i.  `s` is a warp's shared memory, 2 * kMaxDim floats.
+template <typename T>
+__device__ __noinline__ void row_forward(const Args& a, int b, int h, int i, float* s) {
+  const int lane = threadIdx.x & 31, hk = h / a.G;
+  float acc[kDimsPerLane] = {};
+  float m = -INFINITY, l = 0.f;
+  bool any = false;
+  if (i < seq_len(a, b)) {
+    any = true;
+    __syncwarp();
+    stage_row(s, row_ptr<T>(a.q, b, h, i), a.q.s3, a.dqk, lane);
+    __syncwarp();
+    const bool vec = vec_rows<T>(a.k, a.dqk);
+    for_key_chunks(a, i, lane, [&](int j0, uint32_t see) {
+      const float x = see >> lane & 1u ? dot_row(s, row_ptr<T>(a.k, b, hk, j0 + lane), a.k.s3, a.dqk, vec) * a.c2 : -INFINITY;
+      // (a NaN is left to the sums: fmaxf passes over it)
+      const float mn = fmaxf(m, lanes_max(x));
+      const float f = m == mn ? 1.f : exp2f(m - mn);
+      const float p = see >> lane & 1u && x != -INFINITY ? exp2f(x - mn) : 0.f;       // (a row of nothing but -inf: 0 / 0 at the end)
+#pragma unroll
+      for (int t = 0; t < kDimsPerLane; ++t) acc[t] *= f;
+      l = l * f + lanes_sum(p);
+      m = mn;
+      add_rows(acc, p, see, row_ptr<T>(a.v, b, hk, j0), a.v.s2, a.v.s3, a.dv_dim, lane);
+    });
+  }
+  store_row<T>(a.o, b, h, i, acc, any ? 1.f / l : 0.f, a.dv_dim, lane);
+  if (lane == 0) a.lse[((int64_t)b * a.Hq + h) * a.N + i] = any ? m + log2f(l) : -INFINITY;
+}
+
+// dq_i = scale * sum_j p_ij (do_i . v_j - delta_i) k_j
+template <typename T>
+__device__ __noinline__ void row_dq(const Args& a, int b, int h, int i, float* s) {
+  const int lane = threadIdx.x & 31, hk = h / a.G;
+  float acc[kDimsPerLane] = {};
+  if (i < seq_len(a, b)) {
+    __syncwarp();
+    stage_row(s, row_ptr<T>(a.q, b, h, i), a.q.s3, a.dqk, lane);
+    stage_row(s + kMaxDim, row_ptr<T>(a.d_o, b, h, i), a.d_o.s3, a.dv_dim, lane);
+    __syncwarp();
+    const bool kvec = vec_rows<T>(a.k, a.dqk), vvec = vec_rows<T>(a.v, a.dv_dim);
+    const int64_t at = ((int64_t)b * a.Hq + h) * a.N + i;
+    const float lse = a.lse[at], delta = a.delta[at];
+    for_key_chunks(a, i, lane, [&](int j0, uint32_t see) {
+      float ds = 0.f;
+      if (see >> lane & 1u) {
+        const float p = exp2f(dot_row(s, row_ptr<T>(a.k, b, hk, j0 + lane), a.k.s3, a.dqk, kvec) * a.c2 - lse);
+        ds = p * (dot_row(s + kMaxDim, row_ptr<T>(a.v, b, hk, j0 + lane), a.v.s3, a.dv_dim, vvec) - delta);
+      }
+      add_rows(acc, ds, see, row_ptr<T>(a.k, b, hk, j0), a.k.s2, a.k.s3, a.dqk, lane);
+    });
+  }
+  store_row<T>(a.dq, b, h, i, acc, a.scale, a.dqk, lane);
+}
+
+// dk_j = scale * sum_i p_ij (do_i . v_j - delta_i) q_i,  dv_j = sum_i p_ij do_i, over the heads that share key head hk, in order.
+template <typename T>
+__device__ __noinline__ void row_dkdv(const Args& a, int b, int hk, int j, float* s) {
+  const int lane = threadIdx.x & 31, len = seq_len(a, b);
+  float dk[kDimsPerLane] = {}, dv[kDimsPerLane] = {};
+  if (j < len) {
+    __syncwarp();
+    stage_row(s, row_ptr<T>(a.k, b, hk, j), a.k.s3, a.dqk, lane);
+    stage_row(s + kMaxDim, row_ptr<T>(a.v, b, hk, j), a.v.s3, a.dv_dim, lane);
+    __syncwarp();
+    const bool qvec = vec_rows<T>(a.q, a.dqk), ovec = vec_rows<T>(a.d_o, a.dv_dim);
+    const int end = j < a.ns ? len : (int)min((int64_t)len, (int64_t)j + a.W);
+    for (int g = 0; g < a.G; ++g) {
+      const int h = hk * a.G + g;
+      const int64_t at = ((int64_t)b * a.Hq + h) * a.N;
+      for (int i0 = j; i0 < end; i0 += 32) {
+        const uint32_t see = __ballot_sync(0xffffffffu, i0 + lane < end);
+        float p = 0.f, ds = 0.f;
+        if (see >> lane & 1u) {
+          p = exp2f(dot_row(s, row_ptr<T>(a.q, b, h, i0 + lane), a.q.s3, a.dqk, qvec) * a.c2 - a.lse[at + i0 + lane]);
+          ds = p * (dot_row(s + kMaxDim, row_ptr<T>(a.d_o, b, h, i0 + lane), a.d_o.s3, a.dv_dim, ovec) - a.delta[at + i0 + lane]);
+        }
+        add_rows(dv, p, see, row_ptr<T>(a.d_o, b, h, i0), a.d_o.s2, a.d_o.s3, a.dv_dim, lane);
+        add_rows(dk, ds, see, row_ptr<T>(a.q, b, h, i0), a.q.s2, a.q.s3, a.dqk, lane);
+      }
+    }
+  }
+  store_row<T>(a.dk, b, hk, j, dk, a.scale, a.dqk, lane);
+  store_row<T>(a.dv, b, hk, j, dv, 1.f, a.dv_dim, lane);
+}
+
+// KIND 0 forward, 1 dQ, 2 dK/dV.  grid = (rows / 8, heads, B); 8 warps.
+constexpr int kRowWarps = 8;
+template <typename T, int KIND>
+__global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_constant__ Args a) {
+  __shared__ float s[kRowWarps][2 * kMaxDim];
+  pdl_enter();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5;
+  for (int64_t n = (int64_t)blockIdx.x * kRowWarps + warp; n < a.N; n += (int64_t)gridDim.x * kRowWarps) {
+    if constexpr (KIND == 0) row_forward<T>(a, blockIdx.z, blockIdx.y, (int)n, s[warp]);
+    if constexpr (KIND == 1) row_dq<T>(a, blockIdx.z, blockIdx.y, (int)n, s[warp]);
+    if constexpr (KIND == 2) row_dkdv<T>(a, blockIdx.z, blockIdx.y, (int)n, s[warp]);
+  }
+}
+
+}  // namespace sink
+}  // namespace swa

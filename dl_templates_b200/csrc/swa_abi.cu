@@ -181,6 +181,12 @@ bool launch_simt_tile(int kind, const swa_geom_t* g, const swa_rope_t* rope, con
 
 }  // namespace
 
+namespace swa {
+// For the entries in other files (sink_abi.cu): the thread's error message, the count of launches.
+int abi_fail(int code, const char* msg) { return fail(code, "%s", msg); }
+int abi_launched(const char* what) { return launch_ok(what); }
+}  // namespace swa
+
 extern "C" {
 
 int swa_version(void) { return 2; }

@@ -10,6 +10,7 @@
 #include <ATen/ATen.h>
 #include <ATen/TracerMode.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -25,7 +26,7 @@
 #include <string>
 #include <vector>
 
-#include "../../include/swa2d.h"
+#include "../../include/swa_sequence.h"
 
 namespace {
 
@@ -661,7 +662,7 @@ PyObject* pack(std::initializer_list<Tensor> ts) {
 
 // The `apply` of torch.autograd.Function for TiledSwa, TiledSwaRope2D and TiledSwaPackedQKV: what is no plain_call goes there.
 // (Asked from here: a Python method around the native entry that looks at its answer costs every call 0.4 us.)
-PyObject* g_general[3] = {};
+PyObject* g_general[5] = {};       // (3, 4: RotaryPEAxes and SinkSwa, torch_sequence.h)
 PyObject* general(int i, PyObject* const* args, Py_ssize_t n) {
   TORCH_CHECK(g_general[i], "set_general has not been called");
   return PyObject_Vectorcall(g_general[i], args, (size_t)n, nullptr);
@@ -670,10 +671,10 @@ PyObject* general(int i, PyObject* const* args, Py_ssize_t n) {
 PyObject* py_set_general(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Args a{args, n};
-    for (PyObject*& g : g_general) {
+    for (int i = 0; i < 3; ++i) {
       PyObject* o = a.next();
       Py_INCREF(o);
-      Py_XSETREF(g, o);
+      Py_XSETREF(g_general[i], o);
     }
     a.done();
     Py_RETURN_NONE;
@@ -885,6 +886,8 @@ PyObject* py_poll_status(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+#include "torch_sequence.h"
+
 #define SWA_DEF(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {SWA_DEF("tiled_swa", py_tiled_swa),
                            SWA_DEF("tiled_swa_rope2d", py_tiled_swa_rope2d),
@@ -903,6 +906,14 @@ PyMethodDef g_methods[] = {SWA_DEF("tiled_swa", py_tiled_swa),
                            SWA_DEF("status_words", py_status_words),
                            SWA_DEF("check_status", py_check_status),
                            SWA_DEF("poll_status", py_poll_status),
+                           SWA_DEF("rope_axes", py_rope_axes),
+                           SWA_DEF("rope_axes_to", py_rope_axes_to),
+                           SWA_DEF("sink_swa", py_sink_swa),
+                           SWA_DEF("sink_forward", py_sink_forward),
+                           SWA_DEF("sink_backward", py_sink_backward),
+                           SWA_DEF("kv_append", py_kv_append),
+                           SWA_DEF("sink_decode", py_sink_decode),
+                           SWA_DEF("set_general_sequence", py_set_general_sequence),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_swa2d_torch", nullptr, -1, g_methods};
 
