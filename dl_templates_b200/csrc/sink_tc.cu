@@ -1,12 +1,102 @@
-// Host side of the tcgen05 kernels for attention with a sliding window and sink tokens.
+// Host side of the tcgen05 kernels for attention with a sliding window and sink tokens: which calls they take, tensor maps, launches.
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cstdio>
+#include <cstring>
+#include <type_traits>
+
 #include "sink_tc.cuh"
+#include "sink_tc_fwd.cuh"
+#include "swa_tc.cuh"
 
 namespace swa {
 namespace sink {
 
-const char* tc_unsupported(const sink_geom_t*, const swa_tensor_t* const*, int) { return "not built"; }
-const char* tc_error() { return ""; }
-int tc_fwd(const Args&, int, int32_t*, cudaStream_t) { return -1; }
+namespace {
+
+thread_local char g_err[256] = "";
+constexpr int kSmem = 227 * 1024;
+
+int fail(const char* what, const char* why) {
+  snprintf(g_err, sizeof(g_err), "%s: %s", what, why);
+  return -1;
+}
+
+// (element, token, head, batch) of a [B, H, N, d] tensor; boxes of 64 elements x `rows` tokens, 128-byte swizzle, zero fill.
+bool make_map(CUtensorMap* m, const View4& t, int dtype, int B, int H, int N, int d, int rows) {
+  auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tc::tensor_map_encoder());
+  if (!fn) {
+    fail("tensor map", "cuTensorMapEncodeTiled entry point not available");
+    return false;
+  }
+  cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)N, (cuuint64_t)H, (cuuint64_t)B};
+  cuuint64_t strides[3] = {(cuuint64_t)t.s2 * 2, (cuuint64_t)t.s1 * 2, (cuuint64_t)t.s0 * 2};
+  for (int i = 0; i < 3; ++i)                     // a dimension of extent 1 may carry any stride; give it a legal one
+    if (dims[i + 1] == 1) strides[i] = 16;
+  cuuint32_t box[4] = {64u, (cuuint32_t)rows, 1u, 1u}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = fn(m, dtype == SWA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, t.ptr, dims, strides, box,
+                        estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    snprintf(g_err, sizeof(g_err), "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return false;
+  }
+  return true;
+}
+
+}  // namespace
+
+const char* tc_unsupported(const sink_geom_t* g, const swa_tensor_t* const* ts, int n) {
+  if (g->dtype == SWA_F32) return "fp32";
+  if (g->d_qk % 8 || g->d_v % 8 || g->d_qk > 128 || g->d_v > 128) return "head dims must be multiples of 8 up to 128";
+  if (!(g->sm_scale > 0.f)) return "sm_scale must be positive";
+  if ((int64_t)((g->N + kTile - 1) / kTile) * g->B * g->Hq > (1 << 30)) return "too many tiles";
+  if (n == 8) return "the backward pass has no tensor-core kernels";
+  for (int i = 0; ts && i < n; ++i) {
+    const int64_t* s = ts[i]->stride;
+    const int64_t extent[3] = {g->B, 2, g->N};                   // (heads: of q or of k; a stride of 0 is refused for either)
+    if (s[3] != 1 || (uintptr_t)ts[i]->ptr % 16) return "rows must be contiguous and start on 16-byte boundaries";
+    for (int d = 0; d < 3; ++d)
+      if (extent[d] > 1 && (s[d] <= 0 || s[d] % 8 || s[d] >= (int64_t)1 << 38)) return "strides must be positive multiples of 8";
+  }
+  return nullptr;
+}
+
+const char* tc_error() { return g_err; }
+
+int tc_fwd(const Args& a, int dtype, int32_t* status, cudaStream_t st) {
+  const int qc = (a.dqk + 63) / 64, vc = (a.dv_dim + 63) / 64;
+  FwdParams p;
+  memset(&p, 0, sizeof(p));
+  p.a = a;
+  p.status = status;
+  p.pair_heads = a.G % 2 == 0;
+  const int tiles = (a.N + kTile - 1) / kTile;
+  p.n_y = p.pair_heads ? tiles : (tiles + 1) / 2;
+  p.n_x = p.pair_heads ? a.Hq / 2 : a.Hq;
+  p.n_items = p.n_y * a.B * p.n_x;
+  const int fixed = 2 * qc * (int)kChunk + 1024 + (int)sizeof(FwdShared);
+  p.stages = std::min(4, (kSmem - fixed) / ((qc + vc) * (int)kChunk));
+  const int smem = fixed + p.stages * (qc + vc) * (int)kChunk;
+  CUtensorMap tq, tk, tv;
+  if (!make_map(&tq, a.q, dtype, a.B, a.Hq, a.N, a.dqk, kTile) || !make_map(&tk, a.k, dtype, a.B, a.Hkv, a.N, a.dqk, kTile) ||
+      !make_map(&tv, a.v, dtype, a.B, a.Hkv, a.N, a.dv_dim, kTile))
+    return -1;
+  using Kernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const FwdParams);
+#define ROW(bf) {{sink_fwd_kernel<bf, 1, 1>, sink_fwd_kernel<bf, 1, 2>}, {sink_fwd_kernel<bf, 2, 1>, sink_fwd_kernel<bf, 2, 2>}}
+  static const Kernel table[2][2][2] = {ROW(false), ROW(true)};
+#undef ROW
+  const Kernel kern = table[dtype == SWA_BF16][qc - 1][vc - 1];
+  cudaError_t e = allow_smem((const void*)kern);
+  if (e == cudaSuccess) e = launch_pdl(kern, dim3(std::min(p.n_items, tc::sm_count())), kFwdThreadsS, smem, st, tq, tk, tv, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail("launch", cudaGetErrorString(e));
+  }
+  return 0;
+}
+
 int64_t tc_bwd_scratch(const Args&) { return 0; }
 int tc_bwd(const Args&, int, void*, int32_t*, cudaStream_t, int*) { return -1; }
 

@@ -608,6 +608,7 @@ bool tensor_ok(const swa_tensor_t* t, int B, int H) {
 }  // namespace
 
 const char* last_error() { return g_tc_err; }
+void* tensor_map_encoder() { return reinterpret_cast<void*>(encode_fn()); }
 
 int sm_count() {
   static std::atomic<int> cached[64] = {};

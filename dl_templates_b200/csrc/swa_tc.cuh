@@ -14,6 +14,8 @@ namespace tc {
 const char* unsupported_reason(const swa_geom_t* g, const swa_rope_t* rope, const swa_tensor_t* const* tensors,
                                int n_tensors, int which, bool prerotated = false, bool any8 = false);
 const char* last_error();
+// cuTensorMapEncodeTiled of the driver, or nullptr.
+void* tensor_map_encoder();
 
 // SMs of the current device (148 where there is none to ask), kept per device.
 int sm_count();

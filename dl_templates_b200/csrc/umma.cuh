@@ -232,6 +232,13 @@ __device__ __forceinline__ void tma_load_5d_el(uint32_t el, uint32_t smem_dst, c
       ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(el)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_4d_el(uint32_t el, uint32_t smem_dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %7, 0;\n\t"
+      "@e cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n\t}"
+      ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(el)
+      : "memory");
+}
 __device__ __forceinline__ void tma_prefetch_5d_el(uint32_t el, const CUtensorMap* m, int c0, int c1, int c2, int c3, int c4) {
   asm volatile(
       "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %6, 0;\n\t"
@@ -356,6 +363,15 @@ __device__ __forceinline__ void umma_ss_el(uint32_t el, uint32_t d_tmem, uint64_
       "setp.ne.b32 e, %5, 0;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(el)
+      : "memory");
+}
+__device__ __forceinline__ void umma_ts_el(uint32_t el, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(el)
       : "memory");
 }
 // Arrive on `bar` once every MMA issued so far by this thread has completed.
