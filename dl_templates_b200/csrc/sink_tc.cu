@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "sink_tc.cuh"
+#include "sink_tc_bwd.cuh"
 #include "sink_tc_fwd.cuh"
 #include "swa_tc.cuh"
 
@@ -52,7 +53,6 @@ const char* tc_unsupported(const sink_geom_t* g, const swa_tensor_t* const* ts, 
   if (g->d_qk % 8 || g->d_v % 8 || g->d_qk > 128 || g->d_v > 128) return "head dims must be multiples of 8 up to 128";
   if (!(g->sm_scale > 0.f)) return "sm_scale must be positive";
   if ((int64_t)((g->N + kTile - 1) / kTile) * g->B * g->Hq > (1 << 30)) return "too many tiles";
-  if (n == 8) return "the backward pass has no tensor-core kernels";
   for (int i = 0; ts && i < n; ++i) {
     const int64_t* s = ts[i]->stride;
     const int64_t extent[3] = {g->B, 2, g->N};                   // (heads: of q or of k; a stride of 0 is refused for either)
@@ -97,8 +97,78 @@ int tc_fwd(const Args& a, int dtype, int32_t* status, cudaStream_t st) {
   return 0;
 }
 
-int64_t tc_bwd_scratch(const Args&) { return 0; }
-int tc_bwd(const Args&, int, void*, int32_t*, cudaStream_t, int*) { return -1; }
+namespace {
+
+template <int KIND, int XC, int VC>
+int launch_bwd(const Args& a, int dtype, void* scratch, int32_t* status, cudaStream_t st, BwdParams* out) {
+  using S = BwdShape<KIND, XC, VC>;
+  constexpr int N = S::N, kYStage = (XC + VC) * N * 128, kX = (XC + VC) * (int)kChunk;
+  BwdParams p;
+  memset(&p, 0, sizeof(p));
+  p.a = a;
+  p.status = status;
+  p.n_t = (a.N + kTile - 1) / kTile;
+  const int room = kSmem - 1024 - (int)sizeof(BwdShared);
+  p.xbufs = room - 2 * kX >= 2 * kYStage ? 2 : 1;
+  p.stages = std::min(4, (room - p.xbufs * kX) / kYStage);
+  const int smem = 1024 + (int)sizeof(BwdShared) + p.xbufs * kX + p.stages * kYStage;
+  if constexpr (KIND == 1) {
+    p.n_items = p.n_t * a.B * a.Hq;
+  } else {
+    // An ordinary block streams G (W + 127) rows; blocks with sinks, G N rows, are cut into pieces of that length.
+    p.n_sb = std::min(p.n_t, (a.ns + kTile - 1) / kTile);
+    p.piece_len = a.G * ((kTile - 1 + a.W + N - 1) / N);
+    p.pieces = p.n_sb ? (a.G * ((a.N + N - 1) / N) + p.piece_len - 1) / p.piece_len : 0;
+    p.n_sink_items = p.n_sb * p.pieces * a.B * a.Hkv;
+    p.n_items = p.n_sink_items + (p.n_t - p.n_sb) * a.B * a.Hkv;
+    p.part = (float*)scratch;
+  }
+  *out = p;
+  if (!scratch) return 0;                          // asked for its plan only
+  CUtensorMap txq, txv, tyq, tyv;
+  const bool ok = KIND == 1
+      ? make_map(&txq, a.q, dtype, a.B, a.Hq, a.N, a.dqk, kTile) && make_map(&txv, a.d_o, dtype, a.B, a.Hq, a.N, a.dv_dim, kTile) &&
+            make_map(&tyq, a.k, dtype, a.B, a.Hkv, a.N, a.dqk, N) && make_map(&tyv, a.v, dtype, a.B, a.Hkv, a.N, a.dv_dim, N)
+      : make_map(&txq, a.k, dtype, a.B, a.Hkv, a.N, a.dqk, kTile) && make_map(&txv, a.v, dtype, a.B, a.Hkv, a.N, a.dv_dim, kTile) &&
+            make_map(&tyq, a.q, dtype, a.B, a.Hq, a.N, a.dqk, N) && make_map(&tyv, a.d_o, dtype, a.B, a.Hq, a.N, a.dv_dim, N);
+  if (!ok) return -1;
+  const auto kern = dtype == SWA_BF16 ? sink_bwd_kernel<true, KIND, XC, VC> : sink_bwd_kernel<false, KIND, XC, VC>;
+  cudaError_t e = allow_smem((const void*)kern);
+  if (e == cudaSuccess) e = launch_pdl(kern, dim3(std::min(p.n_items, tc::sm_count())), kFwdThreadsS, smem, st, txq, txv, tyq, tyv, p);
+  if (e == cudaSuccess && KIND == 2 && p.pieces > 1) {
+    const dim3 grid(std::min(p.n_sb * kTile, a.N + kRowWarps - 1) / kRowWarps, a.Hkv, a.B);
+    e = dtype == SWA_BF16 ? launch_pdl(sink_join_kernel<__nv_bfloat16, N>, grid, 32 * kRowWarps, 0, st, p)
+                          : launch_pdl(sink_join_kernel<__half, N>, grid, 32 * kRowWarps, 0, st, p);
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail("launch", cudaGetErrorString(e));
+  }
+  return 0;
+}
+
+template <int KIND>
+int launch_bwd(const Args& a, int dtype, void* scratch, int32_t* status, cudaStream_t st, BwdParams* out) {
+  const int x = a.dqk > 64, v = a.dv_dim > 64;
+  return x ? v ? launch_bwd<KIND, 2, 2>(a, dtype, scratch, status, st, out) : launch_bwd<KIND, 2, 1>(a, dtype, scratch, status, st, out)
+           : v ? launch_bwd<KIND, 1, 2>(a, dtype, scratch, status, st, out) : launch_bwd<KIND, 1, 1>(a, dtype, scratch, status, st, out);
+}
+
+}  // namespace
+
+int64_t tc_bwd_scratch(const Args& a) {
+  BwdParams p;
+  launch_bwd<2>(a, SWA_BF16, nullptr, nullptr, nullptr, &p);
+  return p.pieces > 1 ? (int64_t)a.B * a.Hkv * p.n_sb * p.pieces * kTile * (a.dqk + a.dv_dim) * 4 : 0;
+}
+
+int tc_bwd(const Args& a, int dtype, void* scratch, int32_t* status, cudaStream_t st, int* launches) {
+  BwdParams p;
+  if (launch_bwd<1>(a, dtype, scratch, status, st, &p)) return -1;
+  if (launch_bwd<2>(a, dtype, scratch, status, st, &p)) return -1;
+  *launches = p.pieces > 1 ? 3 : 2;
+  return 0;
+}
 
 }  // namespace sink
 }  // namespace swa

@@ -1,0 +1,559 @@
+// tcgen05 backward kernels of the attention with a sliding window and sink tokens: one template, KIND 1 dQ and KIND 2 dK / dV.
+//
+//   P = exp2(c S - lse),  dP = dO V^T,  dS = P (dP - delta):   dQ = scale dS K;   dV = P^T dO,  dK = scale dS^T Q
+//
+// A CTA (one per SM, 384 threads, persistent) holds a resident tile X of 128 rows -- queries and their dO, or keys and their values --
+// and streams blocks Y of N rows of the other side:  S = X_qk Y_qk^T and dP = X_v Y_v^T (for keys: their transposes), and
+// dQ += dS Y_qk, or dV += P Y_v and dK += dS Y_qk, with P and dS as A operands in tensor memory over the scores they came from.
+// dQ and dK/dV in kernels of their own, seven products where five would do: the fifth of a joint kernel, dQ summed by
+// atomics over the key tiles, would make results depend on the order of CTAs.  Heads that share a key head follow each other
+// in the stream of its dK/dV tile, so that their sum is in a fixed order too.
+//
+//   warp 0      TMA producer      warp 1   issues every MMA      warp 2   (KIND 2) -lse and -delta of the streamed rows
+//   warps 4-11  two groups, one thread per resident row each, on half of a block's columns: P while dP is being made, then dS; at the
+//               end of an item they store the accumulators
+// Tensor memory: two score buffers, one dP buffer, the accumulators; N = 128, 96 (d_qk and d_v on different sides of 64) or 80 (both
+// above; dK/dV only) is what then fits.  The scores of the next block are made while a block's P and dS are, its dP as soon as
+// this block's has been read, and this block's products run behind it.
+//
+// Blocks of dK/dV that hold sinks are seen by every later query: their stream is cut into pieces about as long as another block's, the
+// partial sums go to scratch in fp32 and sink_join_kernel adds them in order.
+//
+// Infinities and NaN: as in the forward kernel, rows of the result that end as one are done again by row_dq / row_dkdv.
+#pragma once
+
+#include "sink_tc_fwd.cuh"
+
+namespace swa {
+namespace sink {
+
+struct BwdParams {
+  Args a;
+  int n_items, stages, xbufs;
+  int n_t;                                      // tiles of 128 resident rows
+  int n_sb, pieces, piece_len, n_sink_items;    // KIND 2: blocks that hold sinks, pieces of each at most, blocks of a piece
+  float* part;                                  // [B, Hkv, n_sb, pieces, 128, d_qk + d_v]
+  int32_t* status;
+};
+
+template <int KIND, int XC, int VC>
+struct BwdShape {
+  static constexpr int N = KIND == 1 || XC + VC == 2 ? 128 : XC + VC == 3 ? 96 : 80;
+  static constexpr int kS = 0, kDP = 2 * N, kAcc = 3 * N;        // tensor memory
+  static constexpr int kAccV = kAcc, kAccQK = KIND == 1 ? kAcc : kAcc + VC * 64;
+  static constexpr int CH = (N / 2 + 15) / 16;                   // 16-column chunks of a group, the first's
+  static_assert(kAccQK + XC * 64 <= 512, "tensor memory");
+};
+
+struct BwdShared {
+  uint64_t x_full[2], x_empty[2], y_full[4], y_empty[4], s_full[2], dp_full, ds_ready, acc_full, acc_empty, vec_full[4], vec_empty[4];
+  float vec[4][2][128];                         // -lse, -delta of the streamed rows
+  uint32_t tmem_base;
+  int abort_flag, bad;
+};
+
+// What an item streams: KIND 1 key blocks, KIND 2 query blocks of the heads that share the key head.
+struct BwdItem {
+  int b, h, x0, len;                            // h: head of the resident rows; x0: their first
+  int nb;                                       // blocks
+  int hi, lo, sb;                               // KIND 1: window's blocks, blocks of sinks below them
+  int per_head, first, piece;                   // KIND 2: blocks of a head, the first of this piece; piece < 0: results go straight out
+};
+
+template <int KIND, int N>
+__device__ __forceinline__ BwdItem bwd_item(const BwdParams& p, int item) {
+  const Args& a = p.a;
+  BwdItem w;
+  if constexpr (KIND == 1) {
+    const int per = a.B * a.Hq, r = item % per;
+    w.b = r / a.Hq;
+    w.h = r % a.Hq;
+    w.x0 = (p.n_t - 1 - item / per) * kTile;
+    w.len = seq_len(a, w.b);
+    w.hi = w.x0 / kTile;
+    w.lo = max(0, w.x0 - a.W + 1) / kTile;
+    w.sb = min((a.ns + kTile - 1) / kTile, w.lo);
+    w.nb = w.x0 < w.len ? w.hi - w.lo + 1 + w.sb : 0;
+    w.piece = -1;
+  } else {
+    const int per = a.B * a.Hkv;
+    int blk, piece = 0;
+    int r;
+    if (item < p.n_sink_items) {
+      r = item % per;
+      piece = item / per % p.pieces;
+      blk = item / per / p.pieces;
+    } else {
+      r = (item - p.n_sink_items) % per;
+      blk = p.n_sb + (item - p.n_sink_items) / per;
+    }
+    w.b = r / a.Hkv;
+    w.h = r % a.Hkv;
+    w.x0 = blk * kTile;
+    w.len = seq_len(a, w.b);
+    const int end = blk < p.n_sb ? w.len : (int)min((int64_t)w.len, (int64_t)w.x0 + kTile - 1 + a.W);
+    w.per_head = w.x0 < w.len ? (end - w.x0 + N - 1) / N : 0;
+    const int all = w.per_head * a.G;
+    w.first = piece * p.piece_len;
+    w.nb = blk < p.n_sb ? max(0, min(p.piece_len, all - w.first)) : all;
+    if (blk >= p.n_sb) w.first = 0;
+    w.piece = blk < p.n_sb && all > p.piece_len ? piece : -1;
+  }
+  return w;
+}
+
+template <bool BF16, int KIND, int XC, int VC>
+__global__ void __launch_bounds__(kFwdThreadsS, 1)
+sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constant__ CUtensorMap tm_xv, const __grid_constant__ CUtensorMap tm_yqk,
+                const __grid_constant__ CUtensorMap tm_yv, const __grid_constant__ BwdParams p) {
+  using namespace ptx;
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  using S = BwdShape<KIND, XC, VC>;
+  constexpr int N = S::N, CH = S::CH;
+  constexpr uint32_t kY = N * 128, kYStage = (XC + VC) * kY, kX = (XC + VC) * kChunk;      // bytes: chunk of a block, block, resident tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const Args& a = p.a;
+  uint8_t* x_smem = smem;                                        // buffer: qk chunks, v chunks
+  uint8_t* y_smem = x_smem + p.xbufs * kX;
+  BwdShared* sh = reinterpret_cast<BwdShared*>(y_smem + p.stages * kYStage);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x < offsetof(BwdShared, vec) / 8) {
+    uint64_t* bar = reinterpret_cast<uint64_t*>(sh) + threadIdx.x;
+    mbar_init(bar, bar == &sh->ds_ready || bar == &sh->acc_empty || (bar >= sh->vec_empty && bar < sh->vec_empty + 4) ? 8 : 1);
+  }
+  if (threadIdx.x == 0) sh->abort_flag = sh->bad = 0;
+  fence_barrier_init();
+  if (warp == 1) {
+    tmem_alloc(&sh->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_enter();
+  pdl_wait();
+  const uint32_t tmem = sh->tmem_base;
+  bool ok = true;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { ok &= __all_sync(0xffffffffu, mbar_wait_polls<0>(smem_u32(bar), parity)) != 0; };
+  // first row and head of a streamed block; its columns that count (KIND 1: of a block of sinks below the window only the sinks)
+  auto y_row = [&](const BwdItem& w, int n) {
+    if constexpr (KIND == 1) return (n <= w.hi - w.lo ? w.hi - n : w.sb - 1 - (n - (w.hi - w.lo + 1))) * kTile;
+    else return w.x0 + (w.first + n) % w.per_head * N;
+  };
+  auto y_head = [&](const BwdItem& w, int n) {
+    if constexpr (KIND == 1) return w.h / a.G;
+    else return w.h * a.G + (w.first + n) / w.per_head;
+  };
+  auto y_cols = [&](const BwdItem& w, int n) {
+    if constexpr (KIND == 1) return n <= w.hi - w.lo ? N : min(N, (a.ns - y_row(w, n) + 15) & ~15);
+    else return N;
+  };
+
+  if (warp < 4) {
+    setmaxnreg_dec<72>();
+    if (warp == 0) {
+      // ---------------------------------------------------------------- producer
+      const uint32_t el = elect_one();
+      int st = 0, par = 1, xb = 0, x_par = 1;
+      for (int item = blockIdx.x; ok && item < p.n_items; item += gridDim.x) {
+        const BwdItem w = bwd_item<KIND, N>(p, item);
+        if (!w.nb) continue;
+        wait(&sh->x_empty[xb], x_par);
+        if (!ok) break;
+        const uint32_t xs = smem_u32(x_smem) + xb * kX, xbar = smem_u32(&sh->x_full[xb]);
+        mbar_expect_tx_el(el, xbar, kX);
+#pragma unroll
+        for (int c = 0; c < XC; ++c) tma_load_4d_el(el, xs + c * kChunk, &tm_xqk, xbar, 64 * c, w.x0, w.h, w.b);
+#pragma unroll
+        for (int c = 0; c < VC; ++c) tma_load_4d_el(el, xs + (XC + c) * kChunk, &tm_xv, xbar, 64 * c, w.x0, w.h, w.b);
+        if (++xb == p.xbufs) { xb = 0; x_par ^= 1; }
+        for (int n = 0; n < w.nb; ++n) {
+          const int row = y_row(w, n), h = y_head(w, n);
+          wait(&sh->y_empty[st], par);
+          if (!ok) break;
+          const uint32_t ys = smem_u32(y_smem) + st * kYStage, ybar = smem_u32(&sh->y_full[st]);
+          mbar_expect_tx_el(el, ybar, kYStage);
+#pragma unroll
+          for (int c = 0; c < XC; ++c) tma_load_4d_el(el, ys + c * kY, &tm_yqk, ybar, 64 * c, row, h, w.b);
+#pragma unroll
+          for (int c = 0; c < VC; ++c) tma_load_4d_el(el, ys + (XC + c) * kY, &tm_yv, ybar, 64 * c, row, h, w.b);
+          if (++st == p.stages) { st = 0; par ^= 1; }
+        }
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMA issuer
+      const uint32_t el = elect_one();
+      const uint32_t fmt = BF16 ? 1u : 0u;
+      const uint32_t hi_sw = smem_desc_hi(1024, true);
+      const uint64_t x_d = smem_desc_from(smem_u32(x_smem), 16, hi_sw), y_d = smem_desc_from(smem_u32(y_smem), 16, hi_sw),
+                     ymn_d = smem_desc_from(smem_u32(y_smem), kY, hi_sw);
+      const uint32_t id_qk = instr_desc(fmt, 128, XC * 64, 0, 1), id_v = instr_desc(fmt, 128, VC * 64, 0, 1);
+      int st = 0, y_par = 0, xb = 0, x_par = 0, buf = 0;
+      uint32_t ds_par = 0, acc_par = 1;
+      // (stage and score buffer of the block whose products come next: st, buf)
+      auto scores = [&](int stage, int b2, uint32_t cols) {
+        const uint32_t id = instr_desc(fmt, 128, cols, 0, 0);
+        const uint64_t xd = x_d + (uint64_t)(xb * (kX >> 4)), yd = y_d + (uint64_t)(stage * (kYStage >> 4));
+#pragma unroll
+        for (int k = 0; k < 4 * XC; ++k)
+          umma_ss_el(el, tmem + b2 * N, xd + (k >> 2) * (kChunk >> 4) + 2 * (k & 3), yd + (k >> 2) * (kY >> 4) + 2 * (k & 3), id, k ? 1u : 0u);
+        umma_commit_el(el, &sh->s_full[b2]);
+      };
+      auto dprods = [&](int stage, uint32_t cols) {
+        const uint32_t id = instr_desc(fmt, 128, cols, 0, 0);
+        const uint64_t xd = x_d + (uint64_t)((xb * kX + XC * kChunk) >> 4), yd = y_d + (uint64_t)((stage * kYStage + XC * kY) >> 4);
+#pragma unroll
+        for (int k = 0; k < 4 * VC; ++k)
+          umma_ss_el(el, tmem + S::kDP, xd + (k >> 2) * (kChunk >> 4) + 2 * (k & 3), yd + (k >> 2) * (kY >> 4) + 2 * (k & 3), id, k ? 1u : 0u);
+        umma_commit_el(el, &sh->dp_full);
+      };
+      for (int item = blockIdx.x; ok && item < p.n_items; item += gridDim.x) {
+        const BwdItem w = bwd_item<KIND, N>(p, item);
+        if (!w.nb) continue;
+        wait(&sh->x_full[xb], x_par);
+        wait(&sh->y_full[st], y_par);
+        if (!ok) break;
+        tc_fence_after();
+        scores(st, buf, y_cols(w, 0));
+        dprods(st, y_cols(w, 0));
+        if (w.nb == 1) umma_commit_el(el, &sh->x_empty[xb]);
+        for (int n = 0; n < w.nb; ++n) {
+          const bool more = n + 1 < w.nb;
+          int st2 = st + 1, par2 = y_par;
+          if (st2 == p.stages) { st2 = 0; par2 ^= 1; }
+          const uint32_t cols = y_cols(w, n), cols2 = more ? y_cols(w, n + 1) : 0;
+          if (more) {
+            wait(&sh->y_full[st2], par2);
+            if (!ok) break;
+            tc_fence_after();
+            scores(st2, buf ^ 1, cols2);
+          }
+          wait(&sh->ds_ready, ds_par);
+          ds_par ^= 1;
+          if (!ok) break;
+          tc_fence_after();
+          if (more) {
+            dprods(st2, cols2);
+            if (n + 2 == w.nb) umma_commit_el(el, &sh->x_empty[xb]);
+          }
+          if (n == 0) {
+            wait(&sh->acc_empty, acc_par);
+            acc_par ^= 1;
+            if (!ok) break;
+            tc_fence_after();
+          }
+          // a chunk of 16 columns holds 16 P (KIND 2) and 16 dS, packed into 8 columns each
+          const uint32_t s_tm = tmem + buf * N, acc = n ? 1u : 0u;
+          const uint64_t yq = ymn_d + (uint64_t)((st * kYStage) >> 4), yv = yq + (XC * kY >> 4);
+          if constexpr (KIND == 2) {
+#pragma unroll
+            for (int k = 0; k < N / 16; ++k) umma_ts_el(el, tmem + S::kAccV, s_tm + 16 * k, yv + 128 * k, id_v, k ? 1u : acc);
+#pragma unroll
+            for (int k = 0; k < N / 16; ++k) umma_ts_el(el, tmem + S::kAccQK, s_tm + 16 * k + 8, yq + 128 * k, id_qk, k ? 1u : acc);
+          } else if (cols == N) {
+#pragma unroll
+            for (int k = 0; k < N / 16; ++k) umma_ts_el(el, tmem + S::kAccQK, s_tm + 16 * k, yq + 128 * k, id_qk, k ? 1u : acc);
+          } else {
+            for (uint32_t k = 0; k < cols / 16; ++k) umma_ts_el(el, tmem + S::kAccQK, s_tm + 16 * k, yq + 128 * k, id_qk, k ? 1u : acc);
+          }
+          umma_commit_el(el, &sh->y_empty[st]);
+          st = st2;
+          y_par = par2;
+          buf ^= 1;
+        }
+        if (!ok) break;
+        umma_commit_el(el, &sh->acc_full);
+        if (++xb == p.xbufs) { xb = 0; x_par ^= 1; }
+      }
+    } else if (KIND == 2 && warp == 2) {
+      // ---------------------------------------------------------------- softmax statistics of the streamed rows
+      int v = 0, par = 1;
+      for (int item = blockIdx.x; ok && item < p.n_items; item += gridDim.x) {
+        const BwdItem w = bwd_item<KIND, N>(p, item);
+        for (int n = 0; n < w.nb; ++n) {
+          const int row = y_row(w, n);
+          const int64_t at = ((int64_t)w.b * a.Hq + y_head(w, n)) * a.N + row;
+          float l[4], d[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int r = lane + 32 * x;
+            const bool in = r < N && row + r < w.len;
+            l[x] = in ? a.lse[at + r] : INFINITY;                 // a row behind the end: P = exp2(-inf)
+            d[x] = in ? a.delta[at + r] : 0.f;
+          }
+          wait(&sh->vec_empty[v], par);
+          if (!ok) break;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            sh->vec[v][0][lane + 32 * x] = -l[x];
+            sh->vec[v][1][lane + 32 * x] = -d[x];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->vec_full[v]);
+          if (++v == 4) { v = 0; par ^= 1; }
+        }
+      }
+    }
+  } else {
+    setmaxnreg_inc<208>();
+    // ------------------------------------------------------------------ P and dS, one thread per resident row and group
+    const int g = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int c0 = g * CH * 16;                                  // this group's columns: c0 .. c0 + 16 nch
+    const uint64_t c22 = f2_pack(a.c2, a.c2);
+    int buf = 0, v = 0, v_par = 0;
+    uint32_t s_par = 0, dp_par = 0, acc_par = 0;
+    for (int item = blockIdx.x; ok && item < p.n_items; item += gridDim.x) {
+      const BwdItem w = bwd_item<KIND, N>(p, item);
+      const int x = w.x0 + r;
+      float nlse = -INFINITY, ndelta = 0.f;                      // KIND 1: of the thread's query
+      if constexpr (KIND == 1) {
+        if (w.nb && x < w.len) {
+          const int64_t at = ((int64_t)w.b * a.Hq + w.h) * a.N + x;
+          nlse = -a.lse[at];
+          ndelta = -a.delta[at];
+        }
+      }
+      for (int n = 0; n < w.nb; ++n) {
+        const int y0 = y_row(w, n), cols = y_cols(w, n);
+        const int nch = max(0, min(CH, (cols - c0) >> 4));
+        // columns the row sees: cl .. cr, and (KIND 1) those below cs
+        int cl, cr, cs = 0;
+        bool edge;
+        if constexpr (KIND == 1) {
+          cr = min(x < w.len ? x : -1, w.len - 1) - y0;
+          cl = x - a.W + 1 - y0;
+          cs = a.ns - y0;
+          edge = n <= w.hi - w.lo ? y0 + N - 1 > w.x0 || (y0 <= w.x0 + kTile - 1 - a.W && cs < N) || w.x0 + kTile > w.len : cs < cols || w.x0 + kTile > w.len;
+        } else {
+          const int64_t far = (int64_t)max(w.x0, a.ns) + a.W - 1;                       // the first row that is no sink sees no further
+          cl = x - y0;
+          cr = (x < a.ns ? w.len - 1 : (int)min((int64_t)w.len - 1, (int64_t)x + a.W - 1)) - y0;
+          edge = y0 < w.x0 + kTile - 1 || y0 + N > w.len || (w.x0 + kTile > a.ns && y0 + N - 1 > far);
+        }
+        const bool none = __all_sync(0xffffffffu, cr < c0 || cl > c0 + 16 * nch - 1) && (KIND == 2 || cs <= c0);
+        const uint32_t s_tm = lanes + buf * N + c0, d_tm = lanes + S::kDP + c0;
+        if constexpr (KIND == 2) wait(&sh->vec_full[v], v_par);
+        wait(&sh->s_full[buf], s_par >> buf & 1u);
+        s_par ^= 1u << buf;
+        if (!ok) break;
+        tc_fence_after();
+        if (none) {                                              // all of the warp's pairs are hidden
+          wait(&sh->dp_full, dp_par);
+          if (!ok) break;
+          uint32_t zero[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) zero[e] = 0u;
+          for (int i = 0; i < nch; ++i) {
+            if constexpr (KIND == 2) tmem_st16(s_tm + 16 * i, zero);
+            else tmem_st8(s_tm + 16 * i, zero);
+          }
+        } else {
+          float s[16 * CH];
+#pragma unroll
+          for (int i = 0; i < CH; ++i)
+            if (i < nch) tmem_ld16(s_tm + 16 * i, reinterpret_cast<uint32_t*>(s) + 16 * i);
+          tmem_wait_ld();
+          uint32_t see[(CH + 1) / 2];
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < (CH + 1) / 2; ++i) {
+              see[i] = below(cr + 1 - c0, i) & ~below(cl - c0, i);
+              if constexpr (KIND == 1) see[i] |= below(cr + 1 - c0, i) & below(cs - c0, i);
+            }
+#pragma unroll
+            for (int e = 0; e < 16 * CH; ++e)
+              if (!(see[e >> 5] >> (e & 31) & 1u)) s[e] = -INFINITY;
+          }
+          [[maybe_unused]] const float* vec = sh->vec[v][0] + c0;
+#pragma unroll
+          for (int i = 0; i < CH; ++i) {
+            if (i >= nch) break;
+            [[maybe_unused]] uint32_t pw[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              uint64_t nl;
+              if constexpr (KIND == 2) nl = *reinterpret_cast<const uint64_t*>(vec + 16 * i + 2 * e);
+              else nl = f2_pack(nlse, nlse);
+              const float2 y = f2_unpack(f2_fma(f2_pack(s[16 * i + 2 * e], s[16 * i + 2 * e + 1]), c22, nl));
+              s[16 * i + 2 * e] = exp2f(y.x);
+              s[16 * i + 2 * e + 1] = exp2f(y.y);
+              if constexpr (KIND == 2) pw[e] = tc::pack2<BF16>(s[16 * i + 2 * e], s[16 * i + 2 * e + 1]);
+            }
+            if constexpr (KIND == 2) tmem_st8(s_tm + 16 * i, pw);
+          }
+          wait(&sh->dp_full, dp_par);
+          if (!ok) break;
+          tc_fence_after();
+          float d[16 * CH];
+#pragma unroll
+          for (int i = 0; i < CH; ++i)
+            if (i < nch) tmem_ld16(d_tm + 16 * i, reinterpret_cast<uint32_t*>(d) + 16 * i);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < CH; ++i) {
+            if (i >= nch) break;
+            uint32_t pw[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int c = 16 * i + 2 * e;
+              uint64_t nd;
+              if constexpr (KIND == 2) nd = *reinterpret_cast<const uint64_t*>(vec + 128 + c);
+              else nd = f2_pack(ndelta, ndelta);
+              float2 y = f2_unpack(f2_mul(f2_pack(s[c], s[c + 1]), f2_add(f2_pack(d[c], d[c + 1]), nd)));
+              if (edge) {                                        // (0 * what a hidden pair holds)
+                if (!(see[c >> 5] >> (c & 31) & 1u)) y.x = 0.f;
+                if (!(see[c >> 5] >> (c & 31) & 2u)) y.y = 0.f;
+              }
+              pw[e] = tc::pack2<BF16>(y.x, y.y);
+            }
+            tmem_st8(s_tm + 16 * i + (KIND == 2 ? 8 : 0), pw);
+          }
+        }
+        dp_par ^= 1;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sh->ds_ready);
+          if constexpr (KIND == 2) mbar_arrive(&sh->vec_empty[v]);
+        }
+        buf ^= 1;
+        if (++v == 4) { v = 0; v_par ^= 1; }
+      }
+      if (!ok) break;
+      // ---------------------------------------------------------------- store: dQ in halves, dV by group 0 and dK by group 1
+      const bool in = x < a.N, live = x < w.len;
+      const bool is_v = KIND == 2 && g == 0;
+      const int d = is_v ? a.dv_dim : a.dqk, n32 = KIND == 1 ? XC : is_v ? 2 * VC : 2 * XC, col0 = KIND == 1 ? g * XC * 32 : 0;
+      const View4& out = KIND == 1 ? a.dq : is_v ? a.dv : a.dk;
+      T* row = (T*)out.ptr + w.b * out.s0 + w.h * out.s1 + (int64_t)x * out.s2;
+      if (!w.nb) {
+        if (in && w.piece < 0 && (KIND == 1 || w.first == 0))
+          for (int c = col0; c < d && c < col0 + 32 * n32; c += 8) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
+        continue;
+      }
+      wait(&sh->acc_full, acc_par);
+      acc_par ^= 1;
+      if (!ok) break;
+      tc_fence_after();
+      const float f = is_v ? 1.f : a.scale;
+      const uint64_t f2 = f2_pack(f, f);
+      uint64_t z = 0ull;
+      float* part = nullptr;
+      if (KIND == 2 && w.piece >= 0)
+        part = p.part + (((((int64_t)w.b * a.Hkv + w.h) * p.n_sb + w.x0 / kTile) * p.pieces + w.piece) * kTile + r) * (a.dqk + a.dv_dim) + (is_v ? a.dqk : 0);
+      const uint32_t tm = lanes + (is_v ? S::kAccV : S::kAccQK) + col0;
+#pragma unroll 1
+      for (int c = 0; c < n32; ++c) {
+        uint32_t q[32];
+        tmem_ld32(tm + 32 * c, q);
+        tmem_wait_ld();
+        if (c + 1 == n32) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->acc_empty);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int at = col0 + 32 * c + 8 * u;
+          if (part) {
+            if (at < d) {
+              *reinterpret_cast<uint4*>(part + at) = make_uint4(q[8 * u], q[8 * u + 1], q[8 * u + 2], q[8 * u + 3]);
+              *reinterpret_cast<uint4*>(part + at + 4) = make_uint4(q[8 * u + 4], q[8 * u + 5], q[8 * u + 6], q[8 * u + 7]);
+            }
+            continue;
+          }
+          uint32_t wd[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint64_t y = f2_mul(f2_pack(__uint_as_float(q[8 * u + 2 * e]), __uint_as_float(q[8 * u + 2 * e + 1])), f2);
+            z = f2_fma(y, 0ull, z);
+            const float2 yy = f2_unpack(y);
+            wd[e] = live ? tc::pack2<BF16>(yy.x, yy.y) : 0u;
+          }
+          if (in && at < d) *reinterpret_cast<uint4*>(row + at) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
+        }
+      }
+      const float2 zz = f2_unpack(z);
+      if (live && !(zz.x == 0.f && zz.y == 0.f)) sh->bad = 1;
+    }
+  }
+
+  // -------------------------------------------------------------------- teardown (as in the forward kernel)
+  if (!ok) sh->abort_flag = 1;
+  tc_fence_before();
+  __syncthreads();
+  if (*(volatile int*)&sh->abort_flag) {
+#pragma unroll 1
+    for (int n = 0; n < 64; ++n) __nanosleep(1000);
+    if (threadIdx.x == 0) tc::report_abort(p.status, 7 + KIND, 0);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (*(volatile int*)&sh->bad && !*(volatile int*)&sh->abort_flag) {
+    float* s = reinterpret_cast<float*>(smem) + warp * 2 * kMaxDim;
+    for (int item = blockIdx.x; item < p.n_items; item += gridDim.x) {
+      const BwdItem w = bwd_item<KIND, N>(p, item);
+      if (!w.nb || w.piece >= 0) continue;
+#pragma unroll 1
+      for (int i = w.x0 + warp; i < min(w.len, w.x0 + kTile); i += kFwdThreadsS / 32) {
+        bool bad = false;
+        const T* x = row_ptr<T>(KIND == 1 ? a.dq : a.dk, w.b, w.h, i);
+        for (int d = lane; d < a.dqk; d += 32) bad |= !(fabsf(to_f(x[d])) <= 3.0e38f);
+        if constexpr (KIND == 2) {
+          const T* y = row_ptr<T>(a.dv, w.b, w.h, i);
+          for (int d = lane; d < a.dv_dim; d += 32) bad |= !(fabsf(to_f(y[d])) <= 3.0e38f);
+        }
+        if (!__any_sync(0xffffffffu, bad)) continue;
+        if constexpr (KIND == 1) row_dq<T>(a, w.b, w.h, i, s);
+        else row_dkdv<T>(a, w.b, w.h, i, s);
+      }
+    }
+  }
+}
+
+// dK and dV of the rows of blocks with sinks, from the partial sums of their pieces; one warp per row.
+template <typename T, int N>
+__global__ void __launch_bounds__(32 * kRowWarps) sink_join_kernel(const __grid_constant__ BwdParams p) {
+  __shared__ float smem[kRowWarps][2 * kMaxDim];
+  pdl_enter();
+  pdl_wait();
+  const Args& a = p.a;
+  const int lane = threadIdx.x & 31, j = blockIdx.x * kRowWarps + (threadIdx.x >> 5), hk = blockIdx.y, b = blockIdx.z;
+  const int len = seq_len(a, b), blk = j / kTile, x0 = blk * kTile;
+  if (j >= a.N || blk >= p.n_sb || x0 >= len) return;            // (a block behind the end: zeros, written by its first piece's item)
+  const int all = (len - x0 + N - 1) / N * a.G;
+  if (all <= p.piece_len) return;                                // went straight out
+  const int pieces = (all + p.piece_len - 1) / p.piece_len, d = a.dqk + a.dv_dim;
+  const float* part = p.part + ((((int64_t)b * a.Hkv + hk) * p.n_sb + blk) * p.pieces * kTile + (j - x0)) * d;
+  float acc[8] = {};
+  for (int x = 0; x < (j < len ? pieces : 0); ++x) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      if (lane + 32 * t < d) acc[t] += part[(int64_t)x * kTile * d + lane + 32 * t];
+  }
+  bool bad = false;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) bad |= lane + 32 * t < d && !(fabsf(acc[t]) <= 3.0e38f);
+  if (__any_sync(0xffffffffu, bad)) {
+    row_dkdv<T>(a, b, hk, j, smem[threadIdx.x >> 5]);
+    return;
+  }
+  T* k = (T*)a.dk.ptr + b * a.dk.s0 + hk * a.dk.s1 + (int64_t)j * a.dk.s2;
+  T* v = (T*)a.dv.ptr + b * a.dv.s0 + hk * a.dv.s1 + (int64_t)j * a.dv.s2;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    const int c = lane + 32 * t;
+    if (c < a.dqk) k[c] = from_f<T>(acc[t] * a.scale);
+    else if (c < d) v[c - a.dqk] = from_f<T>(acc[t]);
+  }
+}
+
+}  // namespace sink
+}  // namespace swa
