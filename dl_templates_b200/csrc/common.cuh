@@ -103,21 +103,21 @@ inline cudaError_t launch_pdl(void (*kern)(P...), dim3 grid, unsigned threads, s
   return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
 }
 
-// Set an attribute of a kernel once per kernel and device (the call costs a microsecond).
+// Set an attribute of a kernel once per kernel, attribute and device (the call costs a microsecond).
 inline cudaError_t set_once(const void* kern, cudaFuncAttribute attr, int value) {
-  struct Entry { const void* kern; int dev; };
+  struct Entry { const void* kern; int dev; cudaFuncAttribute attr; };
   static Entry table[512];
   static std::atomic<int> n{0};
   static std::mutex mu;
   int dev = 0;
   if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
   for (int i = 0, have = n.load(std::memory_order_acquire); i < have; ++i)
-    if (table[i].kern == kern && table[i].dev == dev) return cudaSuccess;
+    if (table[i].kern == kern && table[i].dev == dev && table[i].attr == attr) return cudaSuccess;
   std::lock_guard<std::mutex> lock(mu);
   if (cudaError_t e = cudaFuncSetAttribute(kern, attr, value); e != cudaSuccess) return e;
   const int now = n.load();
   if (now < 512) {
-    table[now] = Entry{kern, dev};
+    table[now] = Entry{kern, dev, attr};
     n.store(now + 1, std::memory_order_release);
   }
   return cudaSuccess;

@@ -20,7 +20,7 @@ constexpr int kMaxAxes = 4;
 // Heads of one tensor: `paged` ones go to the pages of a cache [pages, heads, slots, d] instead of a tensor [B, heads, N, d].
 struct Group {
   View4 src, dst;
-  int H, d, rotate, paged, chunks;       // chunks of heads, a blockIdx.y each
+  int H, d, rotate, paged, chunks;       // chunks of heads
 };
 
 struct Args {
@@ -29,7 +29,7 @@ struct Args {
   const float* cs[kMaxAxes];
   const int32_t* pos;                    // element [b, a, n] at b * pos_b + a * pos_a + n
   int64_t pos_b, pos_a;
-  int N;
+  int N, slots;                          // tokens; slots of a row, the widest group's
   float sign;
   const int32_t *page_table, *seq_lens, *new_lens;
   int max_pages, n_pages, page_size;
@@ -57,21 +57,24 @@ __device__ __forceinline__ bool paged_row(const Args& a, const View4& c, int b, 
 
 // One thread: one slot of a token's row in HEADS heads of a group -- VE pairs of an axis, or two units of VE elements that are
 // copied.  The position, the table values and the index arithmetic serve all its heads, and its loads are in flight together.
-// VE elements are what rows, axes and tensors are aligned to, 16 bytes at most.  grid = (slots of all tokens / 256, head chunks, B).
+// VE elements are what rows, axes and tensors are aligned to, 16 bytes at most.  The chunks of heads, tokens and slots of a sequence are one
+// index (a step of one token has 16 slots a head: with a block for each chunk of heads it took 5.5 us, most threads without
+// work), grid = (all of them / 256, 1, B).
 template <typename T, int VE, int HEADS>
 __global__ void __launch_bounds__(256) rotate_kernel(const __grid_constant__ Args a) {
   using U = typename Unit<VE * sizeof(T)>::type;
   pdl_enter();
   pdl_wait();
-  int y = blockIdx.y, gi = 0;
-  while (y >= a.g[gi].chunks) y -= a.g[gi++].chunks;
+  const uint32_t gid = blockIdx.x * 256u + threadIdx.x, row = gid / (uint32_t)a.slots, sl = gid - row * a.slots;
+  const uint32_t chunk = row / (uint32_t)a.N, tok = row - chunk * a.N;
+  int y = (int)chunk, gi = 0;
+  while (gi < 3 && y >= a.g[gi].chunks) y -= a.g[gi++].chunks;
+  if (gi == 3) return;                                           // (no such group: its chunks are 0)
   const Group& g = a.g[gi];
   const int b = blockIdx.z;
   const uint32_t rot_slots = g.rotate ? (uint32_t)a.pairs / VE : 0u;
   const uint32_t spr = rot_slots + (((uint32_t)g.d / VE - 2 * rot_slots + 1) >> 1);
-  const uint32_t gid = blockIdx.x * 256u + threadIdx.x;
-  const uint32_t tok = gid / spr, sl = gid - tok * spr;
-  if (tok >= (uint32_t)a.N) return;
+  if (sl >= spr) return;
   int64_t to = b * g.dst.s0 + (int64_t)tok * g.dst.s2;
   if (g.paged && !paged_row(a, g.dst, b, (int)tok, &to)) return;
   const T* src = (const T*)g.src.ptr + b * g.src.s0 + (int64_t)tok * g.src.s2;

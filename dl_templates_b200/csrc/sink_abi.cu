@@ -147,15 +147,14 @@ int launch_rotate(swa::axes::Args& a, int n_groups, const swa_tensor_t* const* t
     spr = std::max(spr, rot + (a.g[i].d / ve - 2 * rot + 1) / 2);
     heads += a.g[i].H;
   }
-  if (a.N * spr > INT32_MAX) return fail(E_SHAPE, "too many tokens in one call");
-  const int64_t blocks = (a.N * spr + 255) / 256;
   // Four heads a thread where that leaves two blocks for every place on the SMs (8 of 148): their loads are in flight together and the
   // table is read once.
-  const bool four = blocks * B * ((heads + 3) / 4) >= 2 * 8 * 148;
-  unsigned chunks = 0;
+  const bool four = a.N * spr / 256 * B * ((heads + 3) / 4) >= 2 * 8 * 148;
+  int64_t chunks = 0;
   for (int i = 0; i < n_groups; ++i) chunks += a.g[i].chunks = four ? (a.g[i].H + 3) / 4 : a.g[i].H;
-  if (chunks > 65535) return fail(E_SHAPE, "too many heads");
-  const dim3 grid((unsigned)blocks, chunks, B);
+  if (a.N * spr > INT32_MAX || a.N * spr * chunks > INT32_MAX) return fail(E_SHAPE, "too many tokens in one call");
+  a.slots = (int)spr;
+  const dim3 grid((unsigned)((a.N * spr * chunks + 255) / 256), 1, B);
   cudaError_t e = cudaSuccess;
 #define ROT(T, VE) e = four ? swa::launch_stream(swa::axes::rotate_kernel<T, VE, 4>, grid, 256, st, a) : swa::launch_stream(swa::axes::rotate_kernel<T, VE, 1>, grid, 256, st, a)
 #define ROT16(T) do { if (ve == 8) ROT(T, 8); else if (ve == 4) ROT(T, 4); else if (ve == 2) ROT(T, 2); else ROT(T, 1); } while (0)
@@ -193,6 +192,67 @@ int check_cache(const sink_cache_t* c) {
   if (c->n_pages <= 0 || c->page_size <= 0 || c->max_pages <= 0) return fail(E_SHAPE, "pages, page size and table width must be positive");
   if ((int64_t)c->max_pages * c->page_size > (1 << 30)) return fail(E_SHAPE, "a sequence may hold at most 2^30 tokens");
   return 0;
+}
+
+// ---- decode ------------------------------------------------------------------------------------------------------------
+// nullptr when the split kernel takes the call, else the reason it does not.
+const char* split_unsupported(int dtype, const swa::sink::DecodeArgs& a) {
+  const int e = dtype == SWA_F32 ? 4 : 8, esz = 16 / e;
+  if (a.dqk % e || a.dv % e || a.dqk > 128 || a.dv > 128) return "head dims must be multiples of 16 bytes, up to 128 elements";
+  for (const swa::View4* c : {&a.k, &a.v})
+    if (c->s3 != 1 || (uintptr_t)c->ptr % 16 || c->s0 % e || c->s1 % e || c->s2 % e) return "rows of the cache must be contiguous and start on 16-byte boundaries";
+  if (a.q.s3 != 1 || (uintptr_t)a.q.ptr % (2 * esz) || a.q.s0 % 2 || a.q.s1 % 2) return "rows of q must be contiguous and start on even elements";
+  for (const swa::View4* c : {&a.k, &a.v})
+    if (c->s0 > INT32_MAX || c->s2 > INT32_MAX) return "pages of the cache are too far apart";
+  if ((int64_t)a.B * a.Hkv * ((a.G + 15) / 16) > (1 << 26)) return "too many sequences and heads";
+  return nullptr;
+}
+
+template <typename T, int DK, int DV, int HPL>
+cudaError_t launch_split_as(const swa::sink::DecodeArgs& a, unsigned units, cudaStream_t st) {
+  const auto kern = swa::sink::decode_split_kernel<T, DK, DV, HPL>;
+  constexpr int smem = swa::sink::DecodeShape<T, DK, DV>::kSmem;
+  cudaError_t e = swa::set_once((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) e = swa::set_once((const void*)kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess) e = swa::set_once((const void*)kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(units * a.split);
+  cfg.blockDim = dim3(32 * swa::sink::kDecWarps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = a.split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+template <typename T, int HPL>
+cudaError_t launch_split_dims(const swa::sink::DecodeArgs& a, unsigned units, cudaStream_t st) {
+  if (a.dqk <= 64) return a.dv <= 64 ? launch_split_as<T, 64, 64, HPL>(a, units, st) : launch_split_as<T, 64, 128, HPL>(a, units, st);
+  return a.dv <= 64 ? launch_split_as<T, 128, 64, HPL>(a, units, st) : launch_split_as<T, 128, 128, HPL>(a, units, st);
+}
+
+cudaError_t launch_split(int dtype, swa::sink::DecodeArgs& a, cudaStream_t st) {
+  const unsigned units = (unsigned)a.B * a.Hkv * ((a.G + swa::sink::kDecHeads - 1) / swa::sink::kDecHeads);
+  // CTAs of a cluster: as many as fill the GPU's 296 places (two on an SM) once, while every warp keeps two tiles of 16 tokens.
+  // Measured (bf16, d = 128, us with 1 / 2 / 4 / 8 / 16): 8 pairs of sequence and key head, 2052 tokens 25 / 17 / 11.5 / 9.3 / 9.7; 64 pairs,
+  // 6004 tokens 104 / 62 / 41 / 48 / 73; 512 pairs, 4100 tokens 187 / 202 / 213 / 260 / 440.
+  const int64_t seen = std::min((int64_t)a.W + a.ns, (int64_t)a.max_pages * a.page_size);
+  a.split = 1;
+  while (a.split < 16 && (int64_t)units * a.split * 2 <= 2 * 148 + 24 && seen > (int64_t)a.split * swa::sink::kDecWarps * 32) a.split *= 2;
+  a.page_shift = -1;
+  if ((a.page_size & (a.page_size - 1)) == 0)
+    for (a.page_shift = 0; 1 << a.page_shift < a.page_size;) ++a.page_shift;
+  const int nh = std::min(a.G, swa::sink::kDecHeads);
+  if (dtype == SWA_F16) return nh <= 8 ? launch_split_dims<__half, 1>(a, units, st) : launch_split_dims<__half, 2>(a, units, st);
+  if (dtype == SWA_BF16) return nh <= 8 ? launch_split_dims<__nv_bfloat16, 1>(a, units, st) : launch_split_dims<__nv_bfloat16, 2>(a, units, st);
+  return nh <= 4 ? launch_split_dims<float, 1>(a, units, st) : nh <= 8 ? launch_split_dims<float, 2>(a, units, st) : launch_split_dims<float, 4>(a, units, st);
 }
 
 }  // namespace
@@ -348,9 +408,13 @@ int sink_swa_decode(int32_t dtype, int32_t B, int32_t Hq, int32_t Hkv, int32_t d
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.dqk = d_qk; a.dv = d_v; a.W = window; a.ns = n_sink;
   a.max_pages = cache->max_pages; a.n_pages = cache->n_pages; a.page_size = cache->page_size;
   a.c2 = sm_scale * swa::kLog2e;
+  cudaStream_t st = (cudaStream_t)stream;
+  const char* why = split_unsupported(dtype, a);
+  if (impl == SWA_IMPL_TC && (why || dtype == SWA_F32)) return fail(E_IMPL, "tensor-core path unavailable: %s", why ? why : "fp32");
+  if (!why && impl != SWA_IMPL_SIMT) return launched(launch_split(dtype, a, st), "sink decode split");
   const dim3 grid((Hq + swa::sink::kRowWarps - 1) / swa::sink::kRowWarps, B);
   cudaError_t e = cudaSuccess;
-  SINK_DISPATCH(dtype, e = swa::launch_pdl(swa::sink::decode_rows_kernel<T>, grid, 32 * swa::sink::kRowWarps, 0, (cudaStream_t)stream, a));
+  SINK_DISPATCH(dtype, e = swa::launch_pdl(swa::sink::decode_rows_kernel<T>, grid, 32 * swa::sink::kRowWarps, 0, st, a));
   return launched(e, "sink decode");
 }
 
