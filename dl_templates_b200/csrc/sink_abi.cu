@@ -7,6 +7,7 @@
 #include "common.cuh"
 #include "rope_axes.cuh"
 #include "sink_decode.cuh"
+#include "sink_f32.cuh"
 #include "sink_rows.cuh"
 #include "sink_tc.cuh"
 
@@ -116,6 +117,64 @@ int launch_rows(const swa::sink::Args& a, int dtype, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
   SINK_DISPATCH(dtype, e = swa::launch_pdl(swa::sink::rows_kernel<T, KIND>, grid, 32 * swa::sink::kRowWarps, 0, st, a));
   return launched(e, KIND == 0 ? "sink rows forward" : KIND == 1 ? "sink rows dQ" : "sink rows dK/dV");
+}
+
+// ---- fp32 tiles --------------------------------------------------------------------------------------------------------
+bool f32_shape(const sink_geom_t* g) { return g->dtype == SWA_F32 && g->d_qk % 4 == 0 && g->d_v % 4 == 0 && g->d_qk <= 128 && g->d_v <= 128; }
+
+bool f32_tiles(const sink_geom_t* g, const swa_tensor_t* const* ts, int n) {
+  if (!f32_shape(g)) return false;
+  for (int i = 0; i < n; ++i)
+    if (ts[i]->stride[3] != 1 || (uintptr_t)ts[i]->ptr % 16 || ts[i]->stride[0] % 4 || ts[i]->stride[1] % 4 || ts[i]->stride[2] % 4) return false;
+  return true;
+}
+
+// Plan of a kernel: tiles, pieces of the blocks with sinks (KIND 2).  A piece is as long as an ordinary block's stream, G (W + 63) rows.
+template <int KIND>
+swa::sink::F32Params f32_plan(const swa::sink::Args& a, float* part) {
+  constexpr int R = swa::sink::kF32Rows;
+  swa::sink::F32Params p;
+  memset(&p, 0, sizeof(p));
+  p.a = a;
+  p.n_t = (a.N + R - 1) / R;
+  p.part = part;
+  if (KIND == 2) {
+    p.n_sb = std::min(p.n_t, (a.ns + R - 1) / R);
+    p.piece_len = a.G * ((R - 1 + a.W + R - 1) / R);
+    p.pieces = p.n_sb ? (a.G * p.n_t + p.piece_len - 1) / p.piece_len : 0;
+    p.n_sink_items = p.n_sb * p.pieces * a.B * a.Hkv;
+  }
+  return p;
+}
+int64_t f32_scratch(const swa::sink::Args& a) {
+  const swa::sink::F32Params p = f32_plan<2>(a, nullptr);
+  return p.pieces > 1 ? (int64_t)a.B * a.Hkv * p.n_sb * p.pieces * swa::sink::kF32Rows * (a.dqk + a.dv_dim) * 4 : 0;
+}
+
+template <int KIND, int DQ, int DV>
+cudaError_t launch_f32_as(const swa::sink::F32Params& p, int64_t items, cudaStream_t st) {
+  const auto kern = swa::sink::f32_kernel<KIND, DQ, DV>;
+  constexpr int smem = swa::sink::F32Shape<KIND, DQ, DV>::kSmem;
+  cudaError_t e = swa::set_once((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) e = swa::set_once((const void*)kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e != cudaSuccess) return e;
+  kern<<<dim3((unsigned)items), swa::sink::kF32Threads, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <int KIND>
+int launch_f32(const swa::sink::Args& a, float* part, cudaStream_t st) {
+  const swa::sink::F32Params p = f32_plan<KIND>(a, part);
+  const int64_t items = KIND == 2 ? p.n_sink_items + (int64_t)(p.n_t - p.n_sb) * a.B * a.Hkv : (int64_t)p.n_t * a.B * a.Hq;
+  if (items > INT32_MAX) return fail(E_SHAPE, "too many tiles");
+  cudaError_t e = a.dqk <= 64 ? a.dv_dim <= 64 ? launch_f32_as<KIND, 64, 64>(p, items, st) : launch_f32_as<KIND, 64, 128>(p, items, st)
+                              : a.dv_dim <= 64 ? launch_f32_as<KIND, 128, 64>(p, items, st) : launch_f32_as<KIND, 128, 128>(p, items, st);
+  if (int c = launched(e, "sink fp32 tiles")) return c;
+  if (KIND != 2 || p.pieces <= 1) return 0;
+  constexpr int R = swa::sink::kF32Rows, WARPS = swa::sink::kRowWarps;
+  const swa::sink::JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, R, R, part};
+  e = swa::launch_pdl(swa::sink::join_kernel<float>, dim3(std::min(p.n_sb * R, a.N + WARPS - 1) / WARPS, a.Hkv, a.B), 32 * WARPS, 0, st, jp);
+  return launched(e, "sink join");
 }
 
 // ---- rotation --------------------------------------------------------------------------------------------------------
@@ -340,16 +399,21 @@ int sink_swa_fwd(const sink_geom_t* g, const swa_tensor_t* q, const swa_tensor_t
     if (swa::sink::tc_fwd(a, g->dtype, status, st)) return fail(E_LAUNCH, "tcgen05 sink forward: %s", swa::sink::tc_error());
     return abi_launched("tcgen05 sink forward");
   }
+  if (f32_tiles(g, ts, 4)) return launch_f32<0>(a, nullptr, st);
   return launch_rows<0>(a, g->dtype, st);
 }
 
 static int64_t delta_bytes(const sink_geom_t* g) { return ((int64_t)g->B * g->Hq * g->N * 4 + 255) / 256 * 256; }
 
+static int64_t part_bytes(const sink_geom_t* g, int impl) {
+  return impl == SWA_IMPL_TC ? swa::sink::tc_bwd_scratch(make_args(g)) : f32_shape(g) ? f32_scratch(make_args(g)) : 0;
+}
+
 int64_t sink_swa_bwd_scratch(const sink_geom_t* g) {
   if (int e = check_geom(g)) return e;
   const int impl = resolve(g, nullptr, 0);
   if (impl < 0) return impl;
-  return delta_bytes(g) + (impl == SWA_IMPL_TC ? swa::sink::tc_bwd_scratch(make_args(g)) : 0);
+  return delta_bytes(g) + part_bytes(g, impl);
 }
 
 int sink_swa_bwd(const sink_geom_t* g, const swa_tensor_t* q, const swa_tensor_t* k, const swa_tensor_t* v, const swa_tensor_t* o,
@@ -363,7 +427,7 @@ int sink_swa_bwd(const sink_geom_t* g, const swa_tensor_t* q, const swa_tensor_t
   if (!lse || !scratch) return fail(E_NULL, "lse or scratch is NULL");
   const int impl = resolve(g, ts, 8);
   if (impl < 0) return impl;
-  const int64_t need = delta_bytes(g) + (impl == SWA_IMPL_TC ? swa::sink::tc_bwd_scratch(make_args(g)) : 0);
+  const int64_t need = delta_bytes(g) + part_bytes(g, impl);
   if (scratch_bytes < need || (uintptr_t)scratch % 16) return fail(E_SHAPE, "scratch: %lld bytes on a 16-byte boundary needed", (long long)need);
   cudaStream_t st = (cudaStream_t)stream;
   swa::sink::Args a = make_args(g);
@@ -384,6 +448,10 @@ int sink_swa_bwd(const sink_geom_t* g, const swa_tensor_t* q, const swa_tensor_t
     for (int i = 0; i < launches; ++i)
       if (int e = abi_launched("tcgen05 sink backward")) return e;
     return 0;
+  }
+  if (f32_tiles(g, ts, 8)) {
+    if (int e = launch_f32<1>(a, nullptr, st)) return e;
+    return launch_f32<2>(a, (float*)((char*)scratch + delta_bytes(g)), st);
   }
   if (int e = launch_rows<1>(a, g->dtype, st)) return e;
   return launch_rows<2>(a, g->dtype, st);

@@ -205,5 +205,51 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
   }
 }
 
+// ---- dK and dV of blocks with sinks --------------------------------------------------------------------------------------
+// Every later query sees them: the tiled kernels cut the G * ceil((len - x0) / stream) blocks they stream for such a block of `rows` resident
+// rows into pieces of piece_len, each of which leaves its sums in part [B, Hkv, n_sb, pieces, rows, d_qk + d_v].  Added here in the order
+// of the pieces, one warp per row; a block that is a single piece has gone straight out.
+struct JoinParams {
+  Args a;
+  int n_sb, pieces, piece_len, rows, stream;
+  const float* part;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kRowWarps) join_kernel(const __grid_constant__ JoinParams p) {
+  __shared__ float smem[kRowWarps][2 * kMaxDim];
+  pdl_enter();
+  pdl_wait();
+  const Args& a = p.a;
+  const int lane = threadIdx.x & 31, j = blockIdx.x * kRowWarps + (threadIdx.x >> 5), hk = blockIdx.y, b = blockIdx.z;
+  const int len = seq_len(a, b), blk = j / p.rows, x0 = blk * p.rows;
+  if (j >= a.N || blk >= p.n_sb || x0 >= len) return;            // (a block behind the end: zeros, written by its first piece)
+  const int all = (len - x0 + p.stream - 1) / p.stream * a.G;
+  if (all <= p.piece_len) return;
+  const int pieces = (all + p.piece_len - 1) / p.piece_len, d = a.dqk + a.dv_dim;
+  const float* part = p.part + ((((int64_t)b * a.Hkv + hk) * p.n_sb + blk) * p.pieces * p.rows + (j - x0)) * d;
+  float acc[8] = {};
+  for (int x = 0; x < (j < len ? pieces : 0); ++x) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      if (lane + 32 * t < d) acc[t] += part[(int64_t)x * p.rows * d + lane + 32 * t];
+  }
+  bool bad = false;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) bad |= lane + 32 * t < d && !(fabsf(acc[t]) <= 3.0e38f);
+  if (__any_sync(0xffffffffu, bad)) {
+    row_dkdv<T>(a, b, hk, j, smem[threadIdx.x >> 5]);
+    return;
+  }
+  T* k = (T*)a.dk.ptr + b * a.dk.s0 + hk * a.dk.s1 + (int64_t)j * a.dk.s2;
+  T* v = (T*)a.dv.ptr + b * a.dv.s0 + hk * a.dv.s1 + (int64_t)j * a.dv.s2;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    const int c = lane + 32 * t;
+    if (c < a.dqk) k[c * a.dk.s3] = from_f<T>(acc[t] * a.scale);
+    else if (c < d) v[(c - a.dqk) * a.dv.s3] = from_f<T>(acc[t]);
+  }
+}
+
 }  // namespace sink
 }  // namespace swa

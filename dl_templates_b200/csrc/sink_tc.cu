@@ -137,8 +137,9 @@ int launch_bwd(const Args& a, int dtype, void* scratch, int32_t* status, cudaStr
   if (e == cudaSuccess) e = launch_pdl(kern, dim3(std::min(p.n_items, tc::sm_count())), kFwdThreadsS, smem, st, txq, txv, tyq, tyv, p);
   if (e == cudaSuccess && KIND == 2 && p.pieces > 1) {
     const dim3 grid(std::min(p.n_sb * kTile, a.N + kRowWarps - 1) / kRowWarps, a.Hkv, a.B);
-    e = dtype == SWA_BF16 ? launch_pdl(sink_join_kernel<__nv_bfloat16, N>, grid, 32 * kRowWarps, 0, st, p)
-                          : launch_pdl(sink_join_kernel<__half, N>, grid, 32 * kRowWarps, 0, st, p);
+    const JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, kTile, N, p.part};
+    e = dtype == SWA_BF16 ? launch_pdl(join_kernel<__nv_bfloat16>, grid, 32 * kRowWarps, 0, st, jp)
+                          : launch_pdl(join_kernel<__half>, grid, 32 * kRowWarps, 0, st, jp);
   }
   if (e != cudaSuccess) {
     cudaGetLastError();

@@ -17,7 +17,7 @@
 // this block's has been read, and this block's products run behind it.
 //
 // Blocks of dK/dV that hold sinks are seen by every later query: their stream is cut into pieces about as long as another block's, the
-// partial sums go to scratch in fp32 and sink_join_kernel adds them in order.
+// partial sums go to scratch in fp32 and join_kernel (sink_rows.cuh) adds them in order.
 //
 // Infinities and NaN: as in the forward kernel, rows of the result that end as one are done again by row_dq / row_dkdv.
 #pragma once
@@ -515,43 +515,6 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
         else row_dkdv<T>(a, w.b, w.h, i, s);
       }
     }
-  }
-}
-
-// dK and dV of the rows of blocks with sinks, from the partial sums of their pieces; one warp per row.
-template <typename T, int N>
-__global__ void __launch_bounds__(32 * kRowWarps) sink_join_kernel(const __grid_constant__ BwdParams p) {
-  __shared__ float smem[kRowWarps][2 * kMaxDim];
-  pdl_enter();
-  pdl_wait();
-  const Args& a = p.a;
-  const int lane = threadIdx.x & 31, j = blockIdx.x * kRowWarps + (threadIdx.x >> 5), hk = blockIdx.y, b = blockIdx.z;
-  const int len = seq_len(a, b), blk = j / kTile, x0 = blk * kTile;
-  if (j >= a.N || blk >= p.n_sb || x0 >= len) return;            // (a block behind the end: zeros, written by its first piece's item)
-  const int all = (len - x0 + N - 1) / N * a.G;
-  if (all <= p.piece_len) return;                                // went straight out
-  const int pieces = (all + p.piece_len - 1) / p.piece_len, d = a.dqk + a.dv_dim;
-  const float* part = p.part + ((((int64_t)b * a.Hkv + hk) * p.n_sb + blk) * p.pieces * kTile + (j - x0)) * d;
-  float acc[8] = {};
-  for (int x = 0; x < (j < len ? pieces : 0); ++x) {
-#pragma unroll
-    for (int t = 0; t < 8; ++t)
-      if (lane + 32 * t < d) acc[t] += part[(int64_t)x * kTile * d + lane + 32 * t];
-  }
-  bool bad = false;
-#pragma unroll
-  for (int t = 0; t < 8; ++t) bad |= lane + 32 * t < d && !(fabsf(acc[t]) <= 3.0e38f);
-  if (__any_sync(0xffffffffu, bad)) {
-    row_dkdv<T>(a, b, hk, j, smem[threadIdx.x >> 5]);
-    return;
-  }
-  T* k = (T*)a.dk.ptr + b * a.dk.s0 + hk * a.dk.s1 + (int64_t)j * a.dk.s2;
-  T* v = (T*)a.dv.ptr + b * a.dv.s0 + hk * a.dv.s1 + (int64_t)j * a.dv.s2;
-#pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    const int c = lane + 32 * t;
-    if (c < a.dqk) k[c] = from_f<T>(acc[t] * a.scale);
-    else if (c < d) v[c - a.dqk] = from_f<T>(acc[t]);
   }
 }
 
