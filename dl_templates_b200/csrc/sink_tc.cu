@@ -109,7 +109,7 @@ int launch_bwd(const Args& a, int dtype, void* scratch, int32_t* status, cudaStr
   p.status = status;
   p.n_t = (a.N + kTile - 1) / kTile;
   const int room = kSmem - 1024 - (int)sizeof(BwdShared);
-  p.xbufs = room - 2 * kX >= 2 * kYStage ? 2 : 1;
+  p.xbufs = room - 2 * kX >= 3 * kYStage ? 2 : 1;
   p.stages = std::min(4, (room - p.xbufs * kX) / kYStage);
   const int smem = 1024 + (int)sizeof(BwdShared) + p.xbufs * kX + p.stages * kYStage;
   if constexpr (KIND == 1) {

@@ -102,6 +102,42 @@ __device__ __forceinline__ BwdItem bwd_item(const BwdParams& p, int item) {
   return w;
 }
 
+// The blocks of an item one after the other: first row, and head, of each.  (Incremental: with the divisions that find block n from scratch
+// the top of the compute groups' loop took 600 cycles.)
+template <int KIND, int N>
+struct BwdWalk {
+  int y0, h, n, i;                              // i: blocks left of the window (KIND 1), of the head (KIND 2)
+  __device__ __forceinline__ BwdWalk(const BwdItem& w, int G) : n(0) {
+    if constexpr (KIND == 1) {
+      y0 = w.hi * N;
+      h = w.h / G;
+      i = w.hi - w.lo + 1;
+    } else {
+      const int heads = w.first ? w.first / w.per_head : 0, at = w.first - heads * w.per_head;
+      y0 = w.x0 + at * N;
+      h = w.h * G + heads;
+      i = w.per_head - at;
+    }
+  }
+  __device__ __forceinline__ bool window() const { return KIND == 2 || i > 0; }
+  __device__ __forceinline__ int cols(int ns) const { return window() ? N : min(N, (ns - y0 + 15) & ~15); }
+  __device__ __forceinline__ void next(const BwdItem& w) {
+    ++n;
+    --i;
+    if constexpr (KIND == 1) {
+      y0 -= N;
+      if (i == 0) y0 = (w.sb - 1) * N;          // below the window: the blocks of sinks
+    } else {
+      y0 += N;
+      if (i == 0) {
+        y0 = w.x0;
+        ++h;
+        i = w.per_head;
+      }
+    }
+  }
+};
+
 template <bool BF16, int KIND, int XC, int VC>
 __global__ void __launch_bounds__(kFwdThreadsS, 1)
 sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constant__ CUtensorMap tm_xv, const __grid_constant__ CUtensorMap tm_yqk,
@@ -137,19 +173,7 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
   const uint32_t tmem = sh->tmem_base;
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) { ok &= __all_sync(0xffffffffu, mbar_wait_polls<0>(smem_u32(bar), parity)) != 0; };
-  // first row and head of a streamed block; its columns that count (KIND 1: of a block of sinks below the window only the sinks)
-  auto y_row = [&](const BwdItem& w, int n) {
-    if constexpr (KIND == 1) return (n <= w.hi - w.lo ? w.hi - n : w.sb - 1 - (n - (w.hi - w.lo + 1))) * kTile;
-    else return w.x0 + (w.first + n) % w.per_head * N;
-  };
-  auto y_head = [&](const BwdItem& w, int n) {
-    if constexpr (KIND == 1) return w.h / a.G;
-    else return w.h * a.G + (w.first + n) / w.per_head;
-  };
-  auto y_cols = [&](const BwdItem& w, int n) {
-    if constexpr (KIND == 1) return n <= w.hi - w.lo ? N : min(N, (a.ns - y_row(w, n) + 15) & ~15);
-    else return N;
-  };
+  using Walk = BwdWalk<KIND, N>;
 
   if (warp < 4) {
     setmaxnreg_dec<72>();
@@ -169,8 +193,9 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
 #pragma unroll
         for (int c = 0; c < VC; ++c) tma_load_4d_el(el, xs + (XC + c) * kChunk, &tm_xv, xbar, 64 * c, w.x0, w.h, w.b);
         if (++xb == p.xbufs) { xb = 0; x_par ^= 1; }
-        for (int n = 0; n < w.nb; ++n) {
-          const int row = y_row(w, n), h = y_head(w, n);
+        Walk y(w, a.G);
+        for (; y.n < w.nb; y.next(w)) {
+          const int row = y.y0, h = y.h;
           wait(&sh->y_empty[st], par);
           if (!ok) break;
           const uint32_t ys = smem_u32(y_smem) + st * kYStage, ybar = smem_u32(&sh->y_full[st]);
@@ -216,14 +241,17 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
         wait(&sh->y_full[st], y_par);
         if (!ok) break;
         tc_fence_after();
-        scores(st, buf, y_cols(w, 0));
-        dprods(st, y_cols(w, 0));
+        Walk y(w, a.G);
+        uint32_t cols = y.cols(a.ns);
+        scores(st, buf, cols);
+        dprods(st, cols);
         if (w.nb == 1) umma_commit_el(el, &sh->x_empty[xb]);
         for (int n = 0; n < w.nb; ++n) {
           const bool more = n + 1 < w.nb;
           int st2 = st + 1, par2 = y_par;
           if (st2 == p.stages) { st2 = 0; par2 ^= 1; }
-          const uint32_t cols = y_cols(w, n), cols2 = more ? y_cols(w, n + 1) : 0;
+          y.next(w);
+          const uint32_t cols2 = more ? y.cols(a.ns) : 0;
           if (more) {
             wait(&sh->y_full[st2], par2);
             if (!ok) break;
@@ -259,6 +287,7 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
             for (uint32_t k = 0; k < cols / 16; ++k) umma_ts_el(el, tmem + S::kAccQK, s_tm + 16 * k, yq + 128 * k, id_qk, k ? 1u : acc);
           }
           umma_commit_el(el, &sh->y_empty[st]);
+          cols = cols2;
           st = st2;
           y_par = par2;
           buf ^= 1;
@@ -272,9 +301,10 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
       int v = 0, par = 1;
       for (int item = blockIdx.x; ok && item < p.n_items; item += gridDim.x) {
         const BwdItem w = bwd_item<KIND, N>(p, item);
-        for (int n = 0; n < w.nb; ++n) {
-          const int row = y_row(w, n);
-          const int64_t at = ((int64_t)w.b * a.Hq + y_head(w, n)) * a.N + row;
+        if (!w.nb) continue;
+        for (Walk y(w, a.G); y.n < w.nb; y.next(w)) {
+          const int row = y.y0;
+          const int64_t at = ((int64_t)w.b * a.Hq + y.h) * a.N + row;
           float l[4], d[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -309,32 +339,29 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
       const BwdItem w = bwd_item<KIND, N>(p, item);
       const int x = w.x0 + r;
       float nlse = -INFINITY, ndelta = 0.f;                      // KIND 1: of the thread's query
+      // rows of the other side that the thread's row sees: lo .. hi, and (KIND 1) the sinks up to hi
+      int lo, hi;
       if constexpr (KIND == 1) {
+        hi = x < w.len ? x : -1;
+        lo = x - a.W + 1;
         if (w.nb && x < w.len) {
           const int64_t at = ((int64_t)w.b * a.Hq + w.h) * a.N + x;
           nlse = -a.lse[at];
           ndelta = -a.delta[at];
         }
+      } else {
+        lo = x;
+        hi = x < a.ns ? w.len - 1 : (int)min((int64_t)w.len - 1, (int64_t)x + a.W - 1);
       }
-      for (int n = 0; n < w.nb; ++n) {
-        const int y0 = y_row(w, n), cols = y_cols(w, n);
-        const int nch = max(0, min(CH, (cols - c0) >> 4));
-        // columns the row sees: cl .. cr, and (KIND 1) those below cs
-        int cl, cr, cs = 0;
-        bool edge;
-        if constexpr (KIND == 1) {
-          cr = min(x < w.len ? x : -1, w.len - 1) - y0;
-          cl = x - a.W + 1 - y0;
-          cs = a.ns - y0;
-          edge = n <= w.hi - w.lo ? y0 + N - 1 > w.x0 || (y0 <= w.x0 + kTile - 1 - a.W && cs < N) || w.x0 + kTile > w.len : cs < cols || w.x0 + kTile > w.len;
-        } else {
-          const int64_t far = (int64_t)max(w.x0, a.ns) + a.W - 1;                       // the first row that is no sink sees no further
-          cl = x - y0;
-          cr = (x < a.ns ? w.len - 1 : (int)min((int64_t)w.len - 1, (int64_t)x + a.W - 1)) - y0;
-          edge = y0 < w.x0 + kTile - 1 || y0 + N > w.len || (w.x0 + kTile > a.ns && y0 + N - 1 > far);
-        }
-        const bool none = __all_sync(0xffffffffu, cr < c0 || cl > c0 + 16 * nch - 1) && (KIND == 2 || cs <= c0);
+      if (w.nb)
+      for (Walk y(w, a.G); y.n < w.nb; y.next(w)) {
+        const int base = y.y0 + c0, width = 16 * max(0, min(CH, (y.cols(a.ns) - c0) >> 4));
+        // the same as columns of this group, and whether the warp's rows see all of them, or none
+        const int first = lo - base, last = hi - base, sinks = KIND == 1 ? a.ns - base : 0;
+        const bool full = __all_sync(0xffffffffu, last >= width - 1 && (first <= 0 || sinks >= width));
+        const bool none = width == 0 || __all_sync(0xffffffffu, last < 0 || (first >= width && sinks <= 0));
         const uint32_t s_tm = lanes + buf * N + c0, d_tm = lanes + S::kDP + c0;
+        [[maybe_unused]] const float* vec = sh->vec[v][0] + c0;
         if constexpr (KIND == 2) wait(&sh->vec_full[v], v_par);
         wait(&sh->s_full[buf], s_par >> buf & 1u);
         s_par ^= 1u << buf;
@@ -346,71 +373,79 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
           uint32_t zero[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) zero[e] = 0u;
-          for (int i = 0; i < nch; ++i) {
-            if constexpr (KIND == 2) tmem_st16(s_tm + 16 * i, zero);
-            else tmem_st8(s_tm + 16 * i, zero);
+          for (int i = 0; i < width; i += 16) {
+            if constexpr (KIND == 2) tmem_st16(s_tm + i, zero);
+            else tmem_st8(s_tm + i, zero);
           }
         } else {
-          float s[16 * CH];
+          // C chunks of 16 columns: P while dP is being made, then dS.  (A hidden pair has P = 0 and dS = 0 * what it holds.)
+          auto block = [&](auto count) {
+            constexpr int C = decltype(count)::value;
+            float s[16 * C];
 #pragma unroll
-          for (int i = 0; i < CH; ++i)
-            if (i < nch) tmem_ld16(s_tm + 16 * i, reinterpret_cast<uint32_t*>(s) + 16 * i);
-          tmem_wait_ld();
-          uint32_t see[(CH + 1) / 2];
-          if (edge) {
+            for (int i = 0; i < C; ++i) tmem_ld16(s_tm + 16 * i, reinterpret_cast<uint32_t*>(s) + 16 * i);
+            tmem_wait_ld();
+            if (!full) {
+              uint32_t see[(C + 1) / 2];
 #pragma unroll
-            for (int i = 0; i < (CH + 1) / 2; ++i) {
-              see[i] = below(cr + 1 - c0, i) & ~below(cl - c0, i);
-              if constexpr (KIND == 1) see[i] |= below(cr + 1 - c0, i) & below(cs - c0, i);
+              for (int i = 0; i < (C + 1) / 2; ++i) {
+                see[i] = below(last + 1, i) & ~below(first, i);
+                if constexpr (KIND == 1) see[i] |= below(last + 1, i) & below(sinks, i);
+              }
+#pragma unroll
+              for (int e = 0; e < 16 * C; ++e)
+                if (!(see[e >> 5] >> (e & 31) & 1u)) s[e] = -INFINITY;
             }
-#pragma unroll
-            for (int e = 0; e < 16 * CH; ++e)
-              if (!(see[e >> 5] >> (e & 31) & 1u)) s[e] = -INFINITY;
-          }
-          [[maybe_unused]] const float* vec = sh->vec[v][0] + c0;
-#pragma unroll
-          for (int i = 0; i < CH; ++i) {
-            if (i >= nch) break;
             [[maybe_unused]] uint32_t pw[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              uint64_t nl;
-              if constexpr (KIND == 2) nl = *reinterpret_cast<const uint64_t*>(vec + 16 * i + 2 * e);
-              else nl = f2_pack(nlse, nlse);
-              const float2 y = f2_unpack(f2_fma(f2_pack(s[16 * i + 2 * e], s[16 * i + 2 * e + 1]), c22, nl));
-              s[16 * i + 2 * e] = exp2f(y.x);
-              s[16 * i + 2 * e + 1] = exp2f(y.y);
-              if constexpr (KIND == 2) pw[e] = tc::pack2<BF16>(s[16 * i + 2 * e], s[16 * i + 2 * e + 1]);
-            }
-            if constexpr (KIND == 2) tmem_st8(s_tm + 16 * i, pw);
-          }
-          wait(&sh->dp_full, dp_par);
-          if (!ok) break;
-          tc_fence_after();
-          float d[16 * CH];
-#pragma unroll
-          for (int i = 0; i < CH; ++i)
-            if (i < nch) tmem_ld16(d_tm + 16 * i, reinterpret_cast<uint32_t*>(d) + 16 * i);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < CH; ++i) {
-            if (i >= nch) break;
-            uint32_t pw[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int c = 16 * i + 2 * e;
-              uint64_t nd;
-              if constexpr (KIND == 2) nd = *reinterpret_cast<const uint64_t*>(vec + 128 + c);
-              else nd = f2_pack(ndelta, ndelta);
-              float2 y = f2_unpack(f2_mul(f2_pack(s[c], s[c + 1]), f2_add(f2_pack(d[c], d[c + 1]), nd)));
-              if (edge) {                                        // (0 * what a hidden pair holds)
-                if (!(see[c >> 5] >> (c & 31) & 1u)) y.x = 0.f;
-                if (!(see[c >> 5] >> (c & 31) & 2u)) y.y = 0.f;
+            for (int e = 0; e < 8 * C; e += 2) {
+              uint64_t nl[2];
+              if constexpr (KIND == 2) {
+                const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(vec + 2 * e);
+                nl[0] = t.x; nl[1] = t.y;
+              } else {
+                nl[0] = nl[1] = f2_pack(nlse, nlse);
               }
-              pw[e] = tc::pack2<BF16>(y.x, y.y);
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                const float2 t = f2_unpack(f2_fma(f2_pack(s[2 * e + 2 * z], s[2 * e + 2 * z + 1]), c22, nl[z]));
+                s[2 * e + 2 * z] = exp2f(t.x);
+                s[2 * e + 2 * z + 1] = exp2f(t.y);
+                if constexpr (KIND == 2) pw[(e + z) & 7] = tc::pack2<BF16>(s[2 * e + 2 * z], s[2 * e + 2 * z + 1]);
+              }
+              if constexpr (KIND == 2)
+                if ((e & 7) == 6) tmem_st8(s_tm + 2 * (e - 6), pw);
             }
-            tmem_st8(s_tm + 16 * i + (KIND == 2 ? 8 : 0), pw);
-          }
+            wait(&sh->dp_full, dp_par);
+            if (!ok) return;
+            tc_fence_after();
+            float d[16 * C];
+#pragma unroll
+            for (int i = 0; i < C; ++i) tmem_ld16(d_tm + 16 * i, reinterpret_cast<uint32_t*>(d) + 16 * i);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 8 * C; e += 2) {
+              uint64_t nd[2];
+              if constexpr (KIND == 2) {
+                const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(vec + 128 + 2 * e);
+                nd[0] = t.x; nd[1] = t.y;
+              } else {
+                nd[0] = nd[1] = f2_pack(ndelta, ndelta);
+              }
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                const int c = 2 * e + 2 * z;
+                const float2 t = f2_unpack(f2_mul(f2_pack(s[c], s[c + 1]), f2_add(f2_pack(d[c], d[c + 1]), nd[z])));
+                pw[(e + z) & 7] = tc::pack2<BF16>(t.x, t.y);
+              }
+              if ((e & 7) == 6) tmem_st8(s_tm + 2 * (e - 6) + (KIND == 2 ? 8 : 0), pw);
+            }
+          };
+          if (width == 16 * CH) block(std::integral_constant<int, CH>());
+          else if (width == 16 * (CH - 1)) block(std::integral_constant<int, CH - 1>());
+          else if (width == 32) block(std::integral_constant<int, 2>());      // (KIND 1: few sinks)
+          else block(std::integral_constant<int, 1>());
+          if (!ok) break;
         }
         dp_par ^= 1;
         tmem_wait_st();
