@@ -172,7 +172,7 @@ int launch_f32(const swa::sink::Args& a, float* part, cudaStream_t st) {
   if (int c = launched(e, "sink fp32 tiles")) return c;
   if (KIND != 2 || p.pieces <= 1) return 0;
   constexpr int R = swa::sink::kF32Rows, WARPS = swa::sink::kRowWarps;
-  const swa::sink::JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, R, R, part};
+  const swa::sink::JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, R, R, a.dqk + a.dv_dim, 4, part};
   e = swa::launch_pdl(swa::sink::join_kernel<float>, dim3(std::min(p.n_sb * R, a.N + WARPS - 1) / WARPS, a.Hkv, a.B), 32 * WARPS, 0, st, jp);
   return launched(e, "sink join");
 }

@@ -207,11 +207,12 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
 
 // ---- dK and dV of blocks with sinks --------------------------------------------------------------------------------------
 // Every later query sees them: the tiled kernels cut the G * ceil((len - x0) / stream) blocks they stream for such a block of `rows` resident
-// rows into pieces of piece_len, each of which leaves its sums in part [B, Hkv, n_sb, pieces, rows, d_qk + d_v].  Added here in the order
-// of the pieces, one warp per row; a block that is a single piece has gone straight out.
+// rows into pieces of piece_len, each of which leaves its sums in part [B, Hkv, n_sb, pieces, rows * (d_qk + d_v)], row j and column c of
+// them at j * s_row + c / 4 * s_col4 + c % 4.  Added here in the order of the pieces, one warp per row; a block that is a single piece
+// has gone straight out.
 struct JoinParams {
   Args a;
-  int n_sb, pieces, piece_len, rows, stream;
+  int n_sb, pieces, piece_len, rows, stream, s_row, s_col4;
   const float* part;
 };
 
@@ -227,12 +228,13 @@ __global__ void __launch_bounds__(32 * kRowWarps) join_kernel(const __grid_const
   const int all = (len - x0 + p.stream - 1) / p.stream * a.G;
   if (all <= p.piece_len) return;
   const int pieces = (all + p.piece_len - 1) / p.piece_len, d = a.dqk + a.dv_dim;
-  const float* part = p.part + ((((int64_t)b * a.Hkv + hk) * p.n_sb + blk) * p.pieces * p.rows + (j - x0)) * d;
+  const float* part = p.part + (((int64_t)b * a.Hkv + hk) * p.n_sb + blk) * p.pieces * (int64_t)p.rows * d + (j - x0) * p.s_row + (lane >> 2) * p.s_col4 + (lane & 3);
   float acc[8] = {};
+#pragma unroll 4
   for (int x = 0; x < (j < len ? pieces : 0); ++x) {
 #pragma unroll
     for (int t = 0; t < 8; ++t)
-      if (lane + 32 * t < d) acc[t] += part[(int64_t)x * p.rows * d + lane + 32 * t];
+      if (lane + 32 * t < d) acc[t] += part[(int64_t)x * p.rows * d + 8 * t * p.s_col4];
   }
   bool bad = false;
 #pragma unroll

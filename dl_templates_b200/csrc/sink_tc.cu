@@ -24,8 +24,9 @@ int fail(const char* what, const char* why) {
   return -1;
 }
 
-// (element, token, head, batch) of a [B, H, N, d] tensor; boxes of 64 elements x `rows` tokens, 128-byte swizzle, zero fill.
-bool make_map(CUtensorMap* m, const View4& t, int dtype, int B, int H, int N, int d, int rows) {
+// (element, token, head, batch) of a [B, H, N, d] tensor; boxes of `cols` elements x `rows` tokens, swizzled in rows of 128 bytes (cols 64,
+// loads) or 64 (cols 32, stores), zero fill.
+bool make_map(CUtensorMap* m, const View4& t, int dtype, int B, int H, int N, int d, int rows, int cols = 64) {
   auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tc::tensor_map_encoder());
   if (!fn) {
     fail("tensor map", "cuTensorMapEncodeTiled entry point not available");
@@ -35,9 +36,9 @@ bool make_map(CUtensorMap* m, const View4& t, int dtype, int B, int H, int N, in
   cuuint64_t strides[3] = {(cuuint64_t)t.s2 * 2, (cuuint64_t)t.s1 * 2, (cuuint64_t)t.s0 * 2};
   for (int i = 0; i < 3; ++i)                     // a dimension of extent 1 may carry any stride; give it a legal one
     if (dims[i + 1] == 1) strides[i] = 16;
-  cuuint32_t box[4] = {64u, (cuuint32_t)rows, 1u, 1u}, estr[4] = {1, 1, 1, 1};
+  cuuint32_t box[4] = {(cuuint32_t)cols, (cuuint32_t)rows, 1u, 1u}, estr[4] = {1, 1, 1, 1};
   const CUresult r = fn(m, dtype == SWA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, t.ptr, dims, strides, box,
-                        estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        estr, CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     snprintf(g_err, sizeof(g_err), "cuTensorMapEncodeTiled failed (%d)", (int)r);
@@ -65,8 +66,11 @@ const char* tc_unsupported(const sink_geom_t* g, const swa_tensor_t* const* ts, 
 
 const char* tc_error() { return g_err; }
 
-int tc_fwd(const Args& a, int dtype, int32_t* status, cudaStream_t st) {
-  const int qc = (a.dqk + 63) / 64, vc = (a.dv_dim + 63) / 64;
+namespace {
+
+template <int QC, int VC>
+int launch_fwd(const Args& a, int dtype, int32_t* status, cudaStream_t st) {
+  using S = FwdShape<QC, VC>;
   FwdParams p;
   memset(&p, 0, sizeof(p));
   p.a = a;
@@ -76,25 +80,28 @@ int tc_fwd(const Args& a, int dtype, int32_t* status, cudaStream_t st) {
   p.n_y = p.pair_heads ? tiles : (tiles + 1) / 2;
   p.n_x = p.pair_heads ? a.Hq / 2 : a.Hq;
   p.n_items = p.n_y * a.B * p.n_x;
-  const int fixed = 2 * qc * (int)kChunk + 1024 + (int)sizeof(FwdShared);
-  p.stages = std::min(4, (kSmem - fixed) / ((qc + vc) * (int)kChunk));
-  const int smem = fixed + p.stages * (qc + vc) * (int)kChunk;
-  CUtensorMap tq, tk, tv;
-  if (!make_map(&tq, a.q, dtype, a.B, a.Hq, a.N, a.dqk, kTile) || !make_map(&tk, a.k, dtype, a.B, a.Hkv, a.N, a.dqk, kTile) ||
-      !make_map(&tv, a.v, dtype, a.B, a.Hkv, a.N, a.dv_dim, kTile))
+  const int fixed = 2 * QC * (int)kChunk + 1024 + 4 * (int)kStage + (int)sizeof(FwdShared), stage = S::kKStage + S::kVStage;
+  p.stages = std::min(4, (kSmem - fixed) / stage);
+  const int smem = fixed + p.stages * stage;
+  CUtensorMap tq, tk, tv, to;
+  if (!make_map(&tq, a.q, dtype, a.B, a.Hq, a.N, a.dqk, kTile) || !make_map(&tk, a.k, dtype, a.B, a.Hkv, a.N, a.dqk, S::N) ||
+      !make_map(&tv, a.v, dtype, a.B, a.Hkv, a.N, a.dv_dim, S::N) || !make_map(&to, a.o, dtype, a.B, a.Hq, a.N, a.dv_dim, 32, 32))
     return -1;
-  using Kernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const FwdParams);
-#define ROW(bf) {{sink_fwd_kernel<bf, 1, 1>, sink_fwd_kernel<bf, 1, 2>}, {sink_fwd_kernel<bf, 2, 1>, sink_fwd_kernel<bf, 2, 2>}}
-  static const Kernel table[2][2][2] = {ROW(false), ROW(true)};
-#undef ROW
-  const Kernel kern = table[dtype == SWA_BF16][qc - 1][vc - 1];
+  const auto kern = dtype == SWA_BF16 ? sink_fwd_kernel<true, QC, VC> : sink_fwd_kernel<false, QC, VC>;
   cudaError_t e = allow_smem((const void*)kern);
-  if (e == cudaSuccess) e = launch_pdl(kern, dim3(std::min(p.n_items, tc::sm_count())), kFwdThreadsS, smem, st, tq, tk, tv, p);
+  if (e == cudaSuccess) e = launch_pdl(kern, dim3(std::min(p.n_items, tc::sm_count())), kThreads, smem, st, tq, tk, tv, to, p);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail("launch", cudaGetErrorString(e));
   }
   return 0;
+}
+
+}  // namespace
+
+int tc_fwd(const Args& a, int dtype, int32_t* status, cudaStream_t st) {
+  if (a.dqk <= 64) return a.dv_dim <= 64 ? launch_fwd<1, 1>(a, dtype, status, st) : launch_fwd<1, 2>(a, dtype, status, st);
+  return a.dv_dim <= 64 ? launch_fwd<2, 1>(a, dtype, status, st) : launch_fwd<2, 2>(a, dtype, status, st);
 }
 
 namespace {
@@ -108,10 +115,10 @@ int launch_bwd(const Args& a, int dtype, void* scratch, int32_t* status, cudaStr
   p.a = a;
   p.status = status;
   p.n_t = (a.N + kTile - 1) / kTile;
-  const int room = kSmem - 1024 - (int)sizeof(BwdShared);
+  const int room = kSmem - 1024 - 4 * (int)kStage - (int)sizeof(BwdShared);
   p.xbufs = room - 2 * kX >= 3 * kYStage ? 2 : 1;
   p.stages = std::min(4, (room - p.xbufs * kX) / kYStage);
-  const int smem = 1024 + (int)sizeof(BwdShared) + p.xbufs * kX + p.stages * kYStage;
+  const int smem = kSmem - room + p.xbufs * kX + p.stages * kYStage;
   if constexpr (KIND == 1) {
     p.n_items = p.n_t * a.B * a.Hq;
   } else {
@@ -125,19 +132,22 @@ int launch_bwd(const Args& a, int dtype, void* scratch, int32_t* status, cudaStr
   }
   *out = p;
   if (!scratch) return 0;                          // asked for its plan only
-  CUtensorMap txq, txv, tyq, tyv;
-  const bool ok = KIND == 1
+  CUtensorMap txq, txv, tyq, tyv, toq, tov;
+  bool ok = KIND == 1
       ? make_map(&txq, a.q, dtype, a.B, a.Hq, a.N, a.dqk, kTile) && make_map(&txv, a.d_o, dtype, a.B, a.Hq, a.N, a.dv_dim, kTile) &&
             make_map(&tyq, a.k, dtype, a.B, a.Hkv, a.N, a.dqk, N) && make_map(&tyv, a.v, dtype, a.B, a.Hkv, a.N, a.dv_dim, N)
       : make_map(&txq, a.k, dtype, a.B, a.Hkv, a.N, a.dqk, kTile) && make_map(&txv, a.v, dtype, a.B, a.Hkv, a.N, a.dv_dim, kTile) &&
             make_map(&tyq, a.q, dtype, a.B, a.Hq, a.N, a.dqk, N) && make_map(&tyv, a.d_o, dtype, a.B, a.Hq, a.N, a.dv_dim, N);
+  ok = ok && make_map(&toq, KIND == 1 ? a.dq : a.dk, dtype, a.B, KIND == 1 ? a.Hq : a.Hkv, a.N, a.dqk, 32, 32);
+  tov = toq;
+  if (KIND == 2) ok = ok && make_map(&tov, a.dv, dtype, a.B, a.Hkv, a.N, a.dv_dim, 32, 32);
   if (!ok) return -1;
   const auto kern = dtype == SWA_BF16 ? sink_bwd_kernel<true, KIND, XC, VC> : sink_bwd_kernel<false, KIND, XC, VC>;
   cudaError_t e = allow_smem((const void*)kern);
-  if (e == cudaSuccess) e = launch_pdl(kern, dim3(std::min(p.n_items, tc::sm_count())), kFwdThreadsS, smem, st, txq, txv, tyq, tyv, p);
+  if (e == cudaSuccess) e = launch_pdl(kern, dim3(std::min(p.n_items, tc::sm_count())), kThreads, smem, st, txq, txv, tyq, tyv, toq, tov, p);
   if (e == cudaSuccess && KIND == 2 && p.pieces > 1) {
     const dim3 grid(std::min(p.n_sb * kTile, a.N + kRowWarps - 1) / kRowWarps, a.Hkv, a.B);
-    const JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, kTile, N, p.part};
+    const JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, kTile, N, 4, 4 * kTile, p.part};
     e = dtype == SWA_BF16 ? launch_pdl(join_kernel<__nv_bfloat16>, grid, 32 * kRowWarps, 0, st, jp)
                           : launch_pdl(join_kernel<__half>, grid, 32 * kRowWarps, 0, st, jp);
   }

@@ -2,18 +2,20 @@
 //
 //   P = exp2(c S - lse),  dP = dO V^T,  dS = P (dP - delta):   dQ = scale dS K;   dV = P^T dO,  dK = scale dS^T Q
 //
-// A CTA (one per SM, 384 threads, persistent) holds a resident tile X of 128 rows -- queries and their dO, or keys and their values --
+// A CTA (one per SM, persistent) holds a resident tile X of 128 rows -- queries and their dO, or keys and their values --
 // and streams blocks Y of N rows of the other side:  S = X_qk Y_qk^T and dP = X_v Y_v^T (for keys: their transposes), and
 // dQ += dS Y_qk, or dV += P Y_v and dK += dS Y_qk, with P and dS as A operands in tensor memory over the scores they came from.
 // dQ and dK/dV in kernels of their own, seven products where five would do: the fifth of a joint kernel, dQ summed by
 // atomics over the key tiles, would make results depend on the order of CTAs.  Heads that share a key head follow each other
 // in the stream of its dK/dV tile, so that their sum is in a fixed order too.
 //
-//   warp 0      TMA producer      warp 1   issues every MMA      warp 2   (KIND 2) -lse and -delta of the streamed rows
-//   warps 4-11  two groups, one thread per resident row each, on half of a block's columns: P while dP is being made, then dS; at the
-//               end of an item they store the accumulators
-// Tensor memory: two score buffers, one dP buffer, the accumulators; N = 128, 96 (d_qk and d_v on different sides of 64) or 80 (both
-// above; dK/dV only) is what then fits.  The scores of the next block are made while a block's P and dS are, its dP as soon as
+//   warp 0      TMA producer      warp 1   issues every MMA
+//   warp 2      (KIND 2) -lse and -delta of the streamed rows      warp 3   hands out the items (KIND 1: with -lse and -delta of their rows)
+//   warps 4-11  two groups, one thread per resident row each, on half of a block's columns: P while dP is being made, then dS
+//   warps 12-15 epilogue
+// Tensor memory: two score buffers, one dP buffer, the accumulators.  dK/dV: N = 128, 96 (d_qk and d_v on different sides of 64) or 80 (both
+// above) is what then fits; dQ: 128, and 96 with wide heads, whose blocks of 128 leave room for two stages only, so that every load was
+// waited for.  The scores of the next block are made while a block's P and dS are, its dP as soon as
 // this block's has been read, and this block's products run behind it.
 //
 // Blocks of dK/dV that hold sinks are seen by every later query: their stream is cut into pieces about as long as another block's, the
@@ -22,7 +24,7 @@
 // Infinities and NaN: as in the forward kernel, rows of the result that end as one are done again by row_dq / row_dkdv.
 #pragma once
 
-#include "sink_tc_fwd.cuh"
+#include "sink_tc_common.cuh"
 
 namespace swa {
 namespace sink {
@@ -38,27 +40,31 @@ struct BwdParams {
 
 template <int KIND, int XC, int VC>
 struct BwdShape {
-  static constexpr int N = KIND == 1 || XC + VC == 2 ? 128 : XC + VC == 3 ? 96 : 80;
+  static constexpr int N = XC + VC == 2 ? 128 : KIND == 1 ? (XC + VC == 3 ? 128 : 96) : XC + VC == 3 ? 96 : 80;
   static constexpr int kS = 0, kDP = 2 * N, kAcc = 3 * N;        // tensor memory
   static constexpr int kAccV = kAcc, kAccQK = KIND == 1 ? kAcc : kAcc + VC * 64;
   static constexpr int CH = (N / 2 + 15) / 16;                   // 16-column chunks of a group, the first's
   static_assert(kAccQK + XC * 64 <= 512, "tensor memory");
 };
 
-struct BwdShared {
-  uint64_t x_full[2], x_empty[2], y_full[4], y_empty[4], s_full[2], dp_full, ds_ready, acc_full, acc_empty, vec_full[4], vec_empty[4];
-  float vec[4][2][128];                         // -lse, -delta of the streamed rows
-  uint32_t tmem_base;
-  int abort_flag, bad;
-};
-
 // What an item streams: KIND 1 key blocks, KIND 2 query blocks of the heads that share the key head.
 struct BwdItem {
+  int nb;                                       // blocks; -1: no more items
   int b, h, x0, len;                            // h: head of the resident rows; x0: their first
-  int nb;                                       // blocks
   int hi, lo, sb;                               // KIND 1: window's blocks, blocks of sinks below them
   int per_head, first, piece;                   // KIND 2: blocks of a head, the first of this piece; piece < 0: results go straight out
 };
+
+struct BwdShared {
+  uint64_t x_full[2], x_empty[2], y_full[4], y_empty[4], s_full[2], dp_full, ds_ready, acc_full, acc_empty, vec_full[4], vec_empty[4],
+      item_full[kItems], item_empty[kItems];
+  // KIND 2: -lse and -delta of the streamed rows, a ring by blocks; KIND 1: of the resident rows, a ring by items
+  alignas(16) float vec[4][2][kTile];
+  BwdItem item[kItems];
+  uint32_t tmem_base;
+  int abort_flag, bad;
+};
+static_assert(kItems == 4, "vec is a ring of items too");
 
 template <int KIND, int N>
 __device__ __forceinline__ BwdItem bwd_item(const BwdParams& p, int item) {
@@ -70,13 +76,15 @@ __device__ __forceinline__ BwdItem bwd_item(const BwdParams& p, int item) {
     w.h = r % a.Hq;
     w.x0 = (p.n_t - 1 - item / per) * kTile;
     w.len = seq_len(a, w.b);
-    w.hi = w.x0 / kTile;
-    w.lo = max(0, w.x0 - a.W + 1) / kTile;
-    w.sb = min((a.ns + kTile - 1) / kTile, w.lo);
+    w.hi = min(w.x0 + kTile - 1, max(w.len, 1) - 1) / N;
+    w.lo = max(0, w.x0 - a.W + 1) / N;
+    w.sb = min((a.ns + N - 1) / N, w.lo);
     w.nb = w.x0 < w.len ? w.hi - w.lo + 1 + w.sb : 0;
     w.piece = -1;
+    w.first = w.per_head = 0;
   } else {
     const int per = a.B * a.Hkv;
+    w.hi = w.lo = w.sb = 0;
     int blk, piece = 0;
     int r;
     if (item < p.n_sink_items) {
@@ -139,9 +147,10 @@ struct BwdWalk {
 };
 
 template <bool BF16, int KIND, int XC, int VC>
-__global__ void __launch_bounds__(kFwdThreadsS, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constant__ CUtensorMap tm_xv, const __grid_constant__ CUtensorMap tm_yqk,
-                const __grid_constant__ CUtensorMap tm_yv, const __grid_constant__ BwdParams p) {
+                const __grid_constant__ CUtensorMap tm_yv, const __grid_constant__ CUtensorMap tm_oqk, const __grid_constant__ CUtensorMap tm_ov,
+                const __grid_constant__ BwdParams p) {
   using namespace ptx;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   using S = BwdShape<KIND, XC, VC>;
@@ -152,12 +161,15 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
   const Args& a = p.a;
   uint8_t* x_smem = smem;                                        // buffer: qk chunks, v chunks
   uint8_t* y_smem = x_smem + p.xbufs * kX;
-  BwdShared* sh = reinterpret_cast<BwdShared*>(y_smem + p.stages * kYStage);
+  uint8_t* stg_smem = y_smem + p.stages * kYStage;
+  BwdShared* sh = reinterpret_cast<BwdShared*>(stg_smem + 4 * kStage);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x < offsetof(BwdShared, vec) / 8) {
     uint64_t* bar = reinterpret_cast<uint64_t*>(sh) + threadIdx.x;
-    mbar_init(bar, bar == &sh->ds_ready || bar == &sh->acc_empty || (bar >= sh->vec_empty && bar < sh->vec_empty + 4) ? 8 : 1);
+    // consumers of items: producer, issuer, (KIND 2) statistics, 8 warps of the groups, 4 of the epilogue
+    mbar_init(bar, bar == &sh->ds_ready || (bar >= sh->vec_empty && bar < sh->vec_empty + 4) ? 8 : bar == &sh->acc_empty ? 4
+                   : bar >= sh->item_empty && bar < sh->item_empty + kItems ? 13 + KIND : 1);
   }
   if (threadIdx.x == 0) sh->abort_flag = sh->bad = 0;
   fence_barrier_init();
@@ -174,15 +186,30 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) { ok &= __all_sync(0xffffffffu, mbar_wait_polls<0>(smem_u32(bar), parity)) != 0; };
   using Walk = BwdWalk<KIND, N>;
+  // The next item from the ring, its slot in `ii`; done() once nothing of it is read there any more.
+  int ii = kItems - 1, ipar = 1;
+  auto done = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh->item_empty[ii]);
+  };
+  auto take = [&](BwdItem& w, bool keep = false) {
+    if (++ii == kItems) ii = 0;
+    if (ii == 0) ipar ^= 1;
+    wait(&sh->item_full[ii], ipar);
+    if (!ok) return false;
+    w = sh->item[ii];
+    if (!keep || w.nb <= 0) done();
+    return w.nb >= 0;
+  };
 
   if (warp < 4) {
-    setmaxnreg_dec<72>();
+    setmaxnreg_dec<kRegsIssue>();
     if (warp == 0) {
       // ---------------------------------------------------------------- producer
       const uint32_t el = elect_one();
       int st = 0, par = 1, xb = 0, x_par = 1;
-      for (int item = blockIdx.x; ok && item < p.n_items; item += gridDim.x) {
-        const BwdItem w = bwd_item<KIND, N>(p, item);
+      BwdItem w;
+      while (take(w)) {
         if (!w.nb) continue;
         wait(&sh->x_empty[xb], x_par);
         if (!ok) break;
@@ -234,8 +261,8 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
           umma_ss_el(el, tmem + S::kDP, xd + (k >> 2) * (kChunk >> 4) + 2 * (k & 3), yd + (k >> 2) * (kY >> 4) + 2 * (k & 3), id, k ? 1u : 0u);
         umma_commit_el(el, &sh->dp_full);
       };
-      for (int item = blockIdx.x; ok && item < p.n_items; item += gridDim.x) {
-        const BwdItem w = bwd_item<KIND, N>(p, item);
+      BwdItem w;
+      while (take(w)) {
         if (!w.nb) continue;
         wait(&sh->x_full[xb], x_par);
         wait(&sh->y_full[st], y_par);
@@ -299,8 +326,8 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
     } else if (KIND == 2 && warp == 2) {
       // ---------------------------------------------------------------- softmax statistics of the streamed rows
       int v = 0, par = 1;
-      for (int item = blockIdx.x; ok && item < p.n_items; item += gridDim.x) {
-        const BwdItem w = bwd_item<KIND, N>(p, item);
+      BwdItem w;
+      while (take(w)) {
         if (!w.nb) continue;
         for (Walk y(w, a.G); y.n < w.nb; y.next(w)) {
           const int row = y.y0;
@@ -324,19 +351,54 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
           if (lane == 0) mbar_arrive(&sh->vec_full[v]);
           if (++v == 4) { v = 0; par ^= 1; }
         }
+        if (!ok) break;
+      }
+    } else if (warp == 3) {
+      // ---------------------------------------------------------------- items
+      int s = 0, par = 1;
+      for (int item = blockIdx.x; ok; item += gridDim.x) {
+        const bool end = item >= p.n_items;
+        BwdItem w;
+        w.nb = -1;
+        if (!end) w = bwd_item<KIND, N>(p, item);
+        float l[4], d[4];
+        if (KIND == 1 && w.nb > 0) {
+          const int64_t at = ((int64_t)w.b * a.Hq + w.h) * a.N + w.x0;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int r = lane + 32 * x;
+            l[x] = w.x0 + r < w.len ? a.lse[at + r] : INFINITY;
+            d[x] = w.x0 + r < w.len ? a.delta[at + r] : 0.f;
+          }
+        }
+        wait(&sh->item_empty[s], par);
+        if (!ok) break;
+        if (KIND == 1 && w.nb > 0) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            sh->vec[s][0][lane + 32 * x] = -l[x];
+            sh->vec[s][1][lane + 32 * x] = -d[x];
+          }
+        }
+        if (lane == 0) sh->item[s] = w;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->item_full[s]);
+        if (end) break;
+        if (++s == kItems) { s = 0; par ^= 1; }
       }
     }
-  } else {
-    setmaxnreg_inc<208>();
+  } else if (warp < 12) {
+    setmaxnreg_inc<kRegsCompute>();
     // ------------------------------------------------------------------ P and dS, one thread per resident row and group
     const int g = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const int c0 = g * CH * 16;                                  // this group's columns: c0 .. c0 + 16 nch
     const uint64_t c22 = f2_pack(a.c2, a.c2);
     int buf = 0, v = 0, v_par = 0;
-    uint32_t s_par = 0, dp_par = 0, acc_par = 0;
-    for (int item = blockIdx.x; ok && item < p.n_items; item += gridDim.x) {
-      const BwdItem w = bwd_item<KIND, N>(p, item);
+    uint32_t s_par = 0, dp_par = 0;
+    BwdItem w;
+    while (take(w, KIND == 1)) {
+      if (!w.nb) continue;
       const int x = w.x0 + r;
       float nlse = -INFINITY, ndelta = 0.f;                      // KIND 1: of the thread's query
       // rows of the other side that the thread's row sees: lo .. hi, and (KIND 1) the sinks up to hi
@@ -344,16 +406,13 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
       if constexpr (KIND == 1) {
         hi = x < w.len ? x : -1;
         lo = x - a.W + 1;
-        if (w.nb && x < w.len) {
-          const int64_t at = ((int64_t)w.b * a.Hq + w.h) * a.N + x;
-          nlse = -a.lse[at];
-          ndelta = -a.delta[at];
-        }
+        nlse = sh->vec[ii][0][r];
+        ndelta = sh->vec[ii][1][r];
+        done();
       } else {
         lo = x;
         hi = x < a.ns ? w.len - 1 : (int)min((int64_t)w.len - 1, (int64_t)x + a.W - 1);
       }
-      if (w.nb)
       for (Walk y(w, a.G); y.n < w.nb; y.next(w)) {
         const int base = y.y0 + c0, width = 16 * max(0, min(CH, (y.cols(a.ns) - c0) >> 4));
         // the same as columns of this group, and whether the warp's rows see all of them, or none
@@ -416,6 +475,11 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
               if constexpr (KIND == 2)
                 if ((e & 7) == 6) tmem_st8(s_tm + 2 * (e - 6), pw);
             }
+            // (P before the wait, not sunk below it)
+            if constexpr (KIND == 1) {
+#pragma unroll
+              for (int e = 0; e < 16 * C; ++e) asm volatile("" : "+f"(s[e]));
+            }
             wait(&sh->dp_full, dp_par);
             if (!ok) return;
             tc_fence_after();
@@ -459,62 +523,60 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
         if (++v == 4) { v = 0; v_par ^= 1; }
       }
       if (!ok) break;
-      // ---------------------------------------------------------------- store: dQ in halves, dV by group 0 and dK by group 1
-      const bool in = x < a.N, live = x < w.len;
-      const bool is_v = KIND == 2 && g == 0;
-      const int d = is_v ? a.dv_dim : a.dqk, n32 = KIND == 1 ? XC : is_v ? 2 * VC : 2 * XC, col0 = KIND == 1 ? g * XC * 32 : 0;
-      const View4& out = KIND == 1 ? a.dq : is_v ? a.dv : a.dk;
-      T* row = (T*)out.ptr + w.b * out.s0 + w.h * out.s1 + (int64_t)x * out.s2;
+    }
+  } else {
+    setmaxnreg_dec<kRegsEpilogue>();
+    // ------------------------------------------------------------------ epilogue, one thread per resident row
+    const int e = warp & 3, r = e * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(e * 32) << 16);
+    uint8_t* stg = stg_smem + e * kStage;
+    uint32_t par = 0;
+    BwdItem w;
+    while (take(w)) {
+      const int row0 = w.x0 + e * 32;
       if (!w.nb) {
-        if (in && w.piece < 0 && (KIND == 1 || w.first == 0))
-          for (int c = col0; c < d && c < col0 + 32 * n32; c += 8) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
+        if (row0 < a.N && w.piece < 0 && w.first == 0) {
+          store_zeros<BF16>(stg, lane, &tm_oqk, a.dqk, row0, w.h, w.b);
+          if constexpr (KIND == 2) store_zeros<BF16>(stg, lane, &tm_ov, a.dv_dim, row0, w.h, w.b);
+        }
         continue;
       }
-      wait(&sh->acc_full, acc_par);
-      acc_par ^= 1;
+      wait(&sh->acc_full, par);
+      par ^= 1;
       if (!ok) break;
       tc_fence_after();
-      const float f = is_v ? 1.f : a.scale;
-      const uint64_t f2 = f2_pack(f, f);
+      const bool live = w.x0 + r < w.len;
       uint64_t z = 0ull;
-      float* part = nullptr;
-      if (KIND == 2 && w.piece >= 0)
-        part = p.part + (((((int64_t)w.b * a.Hkv + w.h) * p.n_sb + w.x0 / kTile) * p.pieces + w.piece) * kTile + r) * (a.dqk + a.dv_dim) + (is_v ? a.dqk : 0);
-      const uint32_t tm = lanes + (is_v ? S::kAccV : S::kAccQK) + col0;
+      // accumulators, 32 columns at a time: dV, then dQ or dK
+      constexpr int kV = KIND == 2 ? 2 * VC : 0, kAll = kV + 2 * XC;
 #pragma unroll 1
-      for (int c = 0; c < n32; ++c) {
+      for (int c = 0; c < kAll; ++c) {
+        const bool is_v = c < kV;
+        const int col = 32 * (is_v ? c : c - kV);
         uint32_t q[32];
-        tmem_ld32(tm + 32 * c, q);
+        tmem_ld32(lanes + (is_v ? S::kAccV : S::kAccQK) + col, q);
         tmem_wait_ld();
-        if (c + 1 == n32) {
+        if (c + 1 == kAll) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh->acc_empty);
         }
+        if (col >= (is_v ? a.dv_dim : a.dqk)) continue;
+        if (KIND == 2 && w.piece >= 0) {
+          // sums of a piece: [column / 4][row][4], so that a warp's rows lie side by side
+          float* part = p.part + ((((int64_t)w.b * a.Hkv + w.h) * p.n_sb + w.x0 / kTile) * p.pieces + w.piece) * (int64_t)kTile * (a.dqk + a.dv_dim) +
+                        (int64_t)((is_v ? a.dqk : 0) + col) * kTile + r * 4;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int at = col0 + 32 * c + 8 * u;
-          if (part) {
-            if (at < d) {
-              *reinterpret_cast<uint4*>(part + at) = make_uint4(q[8 * u], q[8 * u + 1], q[8 * u + 2], q[8 * u + 3]);
-              *reinterpret_cast<uint4*>(part + at + 4) = make_uint4(q[8 * u + 4], q[8 * u + 5], q[8 * u + 6], q[8 * u + 7]);
-            }
-            continue;
-          }
-          uint32_t wd[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint64_t y = f2_mul(f2_pack(__uint_as_float(q[8 * u + 2 * e]), __uint_as_float(q[8 * u + 2 * e + 1])), f2);
-            z = f2_fma(y, 0ull, z);
-            const float2 yy = f2_unpack(y);
-            wd[e] = live ? tc::pack2<BF16>(yy.x, yy.y) : 0u;
-          }
-          if (in && at < d) *reinterpret_cast<uint4*>(row + at) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
+          for (int u = 0; u < 8; ++u)
+            if (col + 4 * u < (is_v ? a.dv_dim : a.dqk))
+              *reinterpret_cast<uint4*>(part + u * 4 * kTile) = make_uint4(q[4 * u], q[4 * u + 1], q[4 * u + 2], q[4 * u + 3]);
+        } else if (row0 < a.N) {
+          store_columns<BF16>(q, is_v ? 1.f : a.scale, live, z, stg, lane, is_v ? &tm_ov : &tm_oqk, col, row0, w.h, w.b);
         }
       }
-      const float2 zz = f2_unpack(z);
-      if (live && !(zz.x == 0.f && zz.y == 0.f)) sh->bad = 1;
+      if (live && has_nan(z)) sh->bad = 1;
     }
+    if (lane == 0) tma_store_wait_all();
   }
 
   // -------------------------------------------------------------------- teardown (as in the forward kernel)
@@ -537,7 +599,7 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
       const BwdItem w = bwd_item<KIND, N>(p, item);
       if (!w.nb || w.piece >= 0) continue;
 #pragma unroll 1
-      for (int i = w.x0 + warp; i < min(w.len, w.x0 + kTile); i += kFwdThreadsS / 32) {
+      for (int i = w.x0 + warp; i < min(w.len, w.x0 + kTile); i += kThreads / 32) {
         bool bad = false;
         const T* x = row_ptr<T>(KIND == 1 ? a.dq : a.dk, w.b, w.h, i);
         for (int d = lane; d < a.dqk; d += 32) bad |= !(fabsf(to_f(x[d])) <= 3.0e38f);
