@@ -9,13 +9,15 @@
 // (at d = 128 a tile of its own would want 64 bytes a cycle of L2, more than it gives).  The blocks are those of
 // the window, from the diagonal down, then the blocks of sinks the window does not reach, of which only the sinks' columns, in
 // steps of 16, are multiplied.
-//   warp 0       TMA producer: queries, rings of key and value blocks
-//   warp 1       issues every MMA      warp 2   hands out the items
+//   warp 0       TMA producer: queries, rings of key and value blocks      warp 2   hands out the items
+//   warp 1       issues S_t = Q K^T      warp 3   issues O_t += P V   (one warp for both was the bottleneck: 3500 cycles for a
+//                pair of tiles and 80 keys, whose products take 1456)
 //   warps 4-7, 8-11   softmax of tile 0 and 1, one thread per row      warps 12-15   epilogue
-// Tensor memory: S_t, P_t (16-bit, columns of its own), O_t.  With P beside S the scores of the next block are made as soon as a
-// group has taken these into registers, and the groups need not wait for the tensor pipe; with P over S and blocks of 128 a group
-// waited for both products of its tile (2570 cycles a tile and block of d = 128 where the exponentials need 1024 and the products 1024).  What fits
-// beside O: blocks of 128 keys for d_v up to 64, 80 above.
+// Tensor memory: S_t (128 columns), O_t, and P_t (16-bit).  With d_v up to 64 P has columns of its own: the scores of the next block are made as
+// soon as a group has taken these into registers.  Above, P lies over the scores, and the next ones are made when P V is done with
+// it; the two tiles then take turns, one group's exponentials running beside the other tile's products, and P V starts on the first
+// half of P.  (Blocks of 80 keys leave room for P there too, but cost more between blocks: 8192 tokens, window 4096, 16 heads of 128
+// 255 us.)
 // The maximum a row is scaled by is raised only when it has grown by 2^8, so the accumulator is touched rarely.
 //
 // A hidden pair has P = 0, which is nothing to a sum until the value is an infinity or a NaN: a row that ends as one is done again
@@ -49,7 +51,7 @@ struct FwdItem {
 };
 
 struct FwdShared {
-  uint64_t q_full, q_empty, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], s_free[2], p_full[2], pv_done[2], o_full[2], o_empty[2],
+  uint64_t q_full, q_empty, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], s_free[2], p_half[2], p_full[2], pv_done[2], o_full[2], o_empty[2],
       l_full[2], l_empty[2], item_full[kItems], item_empty[kItems];
   FwdItem item[kItems];
   float inv[2][kTile];                          // 1 / l of a tile's rows
@@ -90,10 +92,11 @@ __device__ __forceinline__ int fwd_cols(const Args& a, int blk, int lo) {
 
 template <int QC, int VC>
 struct FwdShape {
-  static constexpr int N = VC == 1 ? 128 : 80;
-  static constexpr uint32_t kP = 2 * N, kO = 512 - 2 * VC * 64;                  // tensor memory: S_t at t N, P_t at kP + t N / 2, O_t
+  static constexpr int N = 128;
+  static constexpr bool kOver = VC > 1;                          // P over S
+  static constexpr uint32_t kP = kOver ? 0 : 2 * N, kPStep = kOver ? N : N / 2, kO = 512 - 2 * VC * 64;     // S_t at t N, P_t at kP + t kPStep, O_t
   static constexpr uint32_t kKStage = QC * N * 128, kVStage = VC * N * 128;
-  static_assert(kP + N <= kO, "tensor memory");
+  static_assert((kOver ? 2 * N : 3 * N) <= kO, "tensor memory");
 };
 
 template <bool BF16, int QC, int VC>
@@ -118,8 +121,8 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   if (threadIdx.x < offsetof(FwdShared, item) / 8) {
     uint64_t* bar = reinterpret_cast<uint64_t*>(sh) + threadIdx.x;
     auto in = [&](uint64_t* x, int n) { return bar >= x && bar < x + n; };
-    const bool warps4 = in(sh->s_free, 2) || in(sh->p_full, 2) || in(sh->o_empty, 2) || in(sh->l_full, 2) || in(sh->l_empty, 2);
-    mbar_init(bar, warps4 ? 4 : in(sh->item_empty, kItems) ? 14 : 1);
+    const bool warps4 = in(sh->s_free, 2) || in(sh->p_half, 2) || in(sh->p_full, 2) || in(sh->o_empty, 2) || in(sh->l_full, 2) || in(sh->l_empty, 2);
+    mbar_init(bar, warps4 ? 4 : in(sh->item_empty, kItems) ? 15 : 1);
   }
   if (threadIdx.x == 0) sh->abort_flag = sh->bad = 0;
   fence_barrier_init();
@@ -183,47 +186,60 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
     } else if (warp == 1) {
-      // ---------------------------------------------------------------- MMA issuer
+      // ---------------------------------------------------------------- scores
       const uint32_t el = elect_one();
       const uint32_t fmt = BF16 ? 1u : 0u;
       const uint32_t hi_sw = smem_desc_hi(1024, true);
-      const uint64_t q_d = smem_desc_from(smem_u32(q_smem), 16, hi_sw), k_d = smem_desc_from(smem_u32(k_smem), 16, hi_sw),
-                     v_d = smem_desc_from(smem_u32(v_smem), kB, hi_sw);
-      const uint32_t id_pv = instr_desc(fmt, 128, kOCols, 0, 1);
-      int ks = 0, kpar = 0, vs = 0, vpar = 0, q_par = 0;
-      uint32_t p_par = 0, o_par = 3, sf_par = 3;                 // a bit per tile
+      const uint64_t q_d = smem_desc_from(smem_u32(q_smem), 16, hi_sw), k_d = smem_desc_from(smem_u32(k_smem), 16, hi_sw);
+      const uint32_t id_full = instr_desc(fmt, 128, N, 0, 0);
+      int ks = 0, kpar = 0, q_par = 0;
+      uint32_t sf_par = 3;                                       // a bit per tile
       FwdItem w;
-      // S_t = Q_t K^T of block blk from key stage ks, once the group has taken the scores before it
-      auto scores = [&](int t, int blk) {
-        wait(&sh->s_free[t], sf_par >> t & 1u);
-        sf_par ^= 1u << t;
-        tc_fence_after();
-        const uint32_t id = instr_desc(fmt, 128, fwd_cols<N>(a, blk, w.lo[t]), 0, 0);
-        const uint64_t qd = q_d + (uint64_t)(t * QC * (kChunk >> 4)), kd = k_d + (uint64_t)(ks * (S::kKStage >> 4));
-#pragma unroll
-        for (int k = 0; k < 4 * QC; ++k)
-          umma_ss_el(el, tmem + t * N, qd + (k >> 2) * (kChunk >> 4) + 2 * (k & 3), kd + (k >> 2) * (kB >> 4) + 2 * (k & 3), id, k ? 1u : 0u);
-        umma_commit_el(el, &sh->s_full[t]);
-      };
       while (take(w)) {
         if (!w.nb) continue;
         wait(&sh->q_full, q_par);
         q_par ^= 1;
-        for (int n = -1; ok && n < w.nb; ++n) {
-          if (n + 1 < w.nb) {                                    // the scores of the next block
-            const int nxt = w.block(n + 1);
-            wait(&sh->k_full[ks], kpar);
+        for (int n = 0; ok && n < w.nb; ++n) {
+          const int blk = w.block(n);
+          wait(&sh->k_full[ks], kpar);
+          const uint64_t kd = k_d + (uint64_t)(ks * (S::kKStage >> 4));
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!w.takes(t, blk)) continue;
+            // the group has taken the scores before, or the product has read the P that lies over them
+            wait(S::kOver ? &sh->pv_done[t] : &sh->s_free[t], sf_par >> t & 1u);
+            sf_par ^= 1u << t;
             if (!ok) break;
             tc_fence_after();
-            for (int t = 0; t < 2; ++t)
-              if (w.takes(t, nxt)) scores(t, nxt);
-            umma_commit_el(el, &sh->k_empty[ks]);
-            if (++ks == p.stages) { ks = 0; kpar ^= 1; }
-            if (n + 2 == w.nb) umma_commit_el(el, &sh->q_empty);
+            const uint32_t id = blk >= w.lo[t] ? id_full : instr_desc(fmt, 128, fwd_cols<N>(a, blk, w.lo[t]), 0, 0);
+            const uint64_t qd = q_d + (uint64_t)(t * QC * (kChunk >> 4));
+#pragma unroll
+            for (int k = 0; k < 4 * QC; ++k)
+              umma_ss_el(el, tmem + t * N, qd + (k >> 2) * (kChunk >> 4) + 2 * (k & 3), kd + (k >> 2) * (kB >> 4) + 2 * (k & 3), id, k ? 1u : 0u);
+            umma_commit_el(el, &sh->s_full[t]);
           }
-          if (n < 0) continue;
+          if (!ok) break;
+          umma_commit_el(el, &sh->k_empty[ks]);
+          if (++ks == p.stages) { ks = 0; kpar ^= 1; }
+        }
+        if (!ok) break;
+        umma_commit_el(el, &sh->q_empty);
+      }
+    } else if (warp == 3) {
+      // ---------------------------------------------------------------- O_t += P_t V
+      const uint32_t el = elect_one();
+      const uint32_t id_pv = instr_desc(BF16 ? 1u : 0u, 128, kOCols, 0, 1);
+      const uint64_t v_d = smem_desc_from(smem_u32(v_smem), kB, smem_desc_hi(1024, true));
+      int vs = 0, vpar = 0;
+      uint32_t p_par = 0, o_par = 3;                             // a bit per tile
+      FwdItem w;
+      while (take(w)) {
+        const int n1[2] = {w.last(0), w.last(1)};
+        for (int n = 0; ok && n < w.nb; ++n) {
           const int blk = w.block(n);
           wait(&sh->v_full[vs], vpar);
+          const uint64_t vd = v_d + (uint64_t)(vs * (S::kVStage >> 4));
+#pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (!w.takes(t, blk)) continue;
             const uint32_t first = n == w.bhi - w.hi[t] ? 0u : 1u;
@@ -231,21 +247,30 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               wait(&sh->o_empty[t], o_par >> t & 1u);
               o_par ^= 1u << t;
             }
+            const uint32_t o_tm = tmem + S::kO + t * kOCols, p_tm = tmem + S::kP + t * S::kPStep;
+            constexpr int kHalf = S::kOver ? N / 32 : 0;         // steps that begin on the first half of P
+            if constexpr (S::kOver) {
+              wait(&sh->p_half[t], p_par >> t & 1u);
+              if (!ok) break;
+              if (blk >= w.lo[t]) {
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < kHalf; ++k) umma_ts_el(el, o_tm, p_tm + 8 * k, vd + 128 * k, id_pv, k ? 1u : first);
+              }
+            }
             wait(&sh->p_full[t], p_par >> t & 1u);
             p_par ^= 1u << t;
             if (!ok) break;
             tc_fence_after();
-            const uint64_t vd = v_d + (uint64_t)(vs * (S::kVStage >> 4));
-            const uint32_t o_tm = tmem + S::kO + t * kOCols, p_tm = tmem + S::kP + t * (N / 2);
-            const int steps = fwd_cols<N>(a, blk, w.lo[t]) >> 4;
-            if (steps == N / 16) {
+            if (blk >= w.lo[t]) {
 #pragma unroll
-              for (int k = 0; k < N / 16; ++k) umma_ts_el(el, o_tm, p_tm + 8 * k, vd + 128 * k, id_pv, k ? 1u : first);
+              for (int k = kHalf; k < N / 16; ++k) umma_ts_el(el, o_tm, p_tm + 8 * k, vd + 128 * k, id_pv, k ? 1u : first);
             } else {
+              const int steps = fwd_cols<N>(a, blk, w.lo[t]) >> 4;
               for (int k = 0; k < steps; ++k) umma_ts_el(el, o_tm, p_tm + 8 * k, vd + 128 * k, id_pv, k ? 1u : first);
             }
             umma_commit_el(el, &sh->pv_done[t]);
-            if (n == w.last(t)) umma_commit_el(el, &sh->o_full[t]);
+            if (n == n1[t]) umma_commit_el(el, &sh->o_full[t]);
           }
           if (!ok) break;
           umma_commit_el(el, &sh->v_empty[vs]);
@@ -276,13 +301,13 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     // ------------------------------------------------------------------ softmax, one thread per row
     const int t = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t s_tm = lanes + t * N, p_tm = lanes + S::kP + t * (N / 2), o_tm = lanes + S::kO + t * kOCols;
+    const uint32_t s_tm = lanes + t * N, p_tm = lanes + S::kP + t * S::kPStep, o_tm = lanes + S::kO + t * kOCols;
     const float c2 = a.c2;
     const uint64_t c22 = f2_pack(c2, c2);
     uint32_t s_par = 0, l_par = 1, pv_par = 0;
     bool pv_open = false;                                        // a product of this tile that has not been waited for
-    auto wait_pv = [&]() {
-      if (!pv_open) return;
+    auto wait_pv = [&]() {                                       // (P over S: these scores came after it)
+      if (S::kOver || !pv_open) return;
       wait(&sh->pv_done[t], pv_par);
       pv_par ^= 1;
       pv_open = false;
@@ -298,9 +323,11 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const int n0 = w.bhi - t_hi, n1 = w.last(t);
       // keys the row sees: lo .. hi, and the sinks
       const int hi = min(i, w.len - 1), lo = i - a.W + 1;
-      for (int n = n0; n <= n1; ++n) {
-        const int blk = w.block(n);
-        if (!(blk <= t_hi && (blk >= t_lo || blk < w.sbn))) continue;
+      const int sbn = w.sbn, nwin = w.nwin, sb = w.sb;
+      int blk = t_hi;
+      for (int n = n0; n <= n1; ++n, --blk) {
+        if (n == nwin) blk = sb - 1;                             // below the window: the blocks of sinks
+        if (blk < t_lo && blk >= sbn) continue;
         const int kb = blk * N, cols = fwd_cols<N>(a, blk, t_lo);
         const int first = lo - kb, last = hi - kb, sinks = a.ns - kb;        // as columns of the block
         const bool full = __all_sync(0xffffffffu, last >= cols - 1 && (first <= 0 || sinks >= cols));
@@ -310,6 +337,7 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         tc_fence_after();
         auto taken = [&]() {                                     // the scores are in registers
           tmem_wait_ld();
+          if constexpr (S::kOver) return;
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh->s_free[t]);
@@ -336,6 +364,12 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (need || m == -INFINITY) m = mx;
         };
         uint64_t ls[2] = {0ull, 0ull};
+        auto half = [&]() {                                      // the first half of P is there
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->p_half[t]);
+        };
         // C chunks of 16 columns
         auto block = [&](auto count) {
           constexpr int C = decltype(count)::value;
@@ -358,6 +392,7 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           grow(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
           const float mc = m == -INFINITY ? 0.f : m * c2;
           const uint64_t nmc2 = f2_pack(-mc, -mc);
+          wait_pv();                                             // the product that read P last
 #pragma unroll
           for (int c = 0; c < C; ++c) {
             uint32_t pw[8];
@@ -368,8 +403,8 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               ls[h & 1] = f2_add(ls[h & 1], f2_pack(p0, p1));
               pw[h] = tc::pack2<BF16>(p0, p1);
             }
-            if (c == 0) wait_pv();                               // the product that read P last
             tmem_st8(p_tm + 8 * c, pw);
+            if (S::kOver && C == N / 16 && c == C / 2 - 1) half();
           }
         };
         if (cols == N) block(std::integral_constant<int, N / 16>());
@@ -407,6 +442,7 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
           taken();
         }
+        if (S::kOver && cols != N) half();
         if (!ok) break;
         const float2 l0 = f2_unpack(ls[0]), l1 = f2_unpack(ls[1]);
         l += (l0.x + l0.y) + (l1.x + l1.y);
