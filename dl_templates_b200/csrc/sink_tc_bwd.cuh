@@ -9,8 +9,8 @@
 // atomics over the key tiles, would make results depend on the order of CTAs.  Heads that share a key head follow each other
 // in the stream of its dK/dV tile, so that their sum is in a fixed order too.
 //
-//   warp 0      TMA producer      warp 1   issues every MMA
-//   warp 2      (KIND 2) -lse and -delta of the streamed rows      warp 3   hands out the items (KIND 1: with -lse and -delta of their rows)
+//   warp 0      TMA producer      warp 1   issues S and dP      warp 3   issues the products of P and dS
+//   warp 2      hands out the items, and -lse and -delta: KIND 1 of an item's rows with it, KIND 2 of the streamed rows block by block
 //   warps 4-11  two groups, one thread per resident row each, on half of a block's columns: P while dP is being made, then dS
 //   warps 12-15 epilogue
 // Tensor memory: two score buffers, one dP buffer, the accumulators.  dK/dV: N = 128, 96 (d_qk and d_v on different sides of 64) or 80 (both
@@ -56,7 +56,9 @@ struct BwdItem {
 };
 
 struct BwdShared {
-  uint64_t x_full[2], x_empty[2], y_full[4], y_empty[4], s_full[2], dp_full, ds_ready, acc_full, acc_empty, vec_full[4], vec_empty[4],
+  // ds_ready: a barrier per score buffer.  Both issuers wait for it, and the second may be behind by a block, waiting for the epilogue; the
+  // next phase of a buffer's barrier needs scores that are made only after the products of the one before (s_done).
+  uint64_t x_full[2], x_empty[2], y_full[4], y_empty[4], s_full[2], s_done[2], ds_ready[2], dp_full, acc_full, acc_empty, vec_full[4], vec_empty[4],
       item_full[kItems], item_empty[kItems];
   // KIND 2: -lse and -delta of the streamed rows, a ring by blocks; KIND 1: of the resident rows, a ring by items
   alignas(16) float vec[4][2][kTile];
@@ -167,9 +169,9 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
 
   if (threadIdx.x < offsetof(BwdShared, vec) / 8) {
     uint64_t* bar = reinterpret_cast<uint64_t*>(sh) + threadIdx.x;
-    // consumers of items: producer, issuer, (KIND 2) statistics, 8 warps of the groups, 4 of the epilogue
-    mbar_init(bar, bar == &sh->ds_ready || (bar >= sh->vec_empty && bar < sh->vec_empty + 4) ? 8 : bar == &sh->acc_empty ? 4
-                   : bar >= sh->item_empty && bar < sh->item_empty + kItems ? 13 + KIND : 1);
+    // consumers of items: producer, two issuers, 8 warps of the groups, 4 of the epilogue
+    mbar_init(bar, (bar >= sh->ds_ready && bar < sh->ds_ready + 2) || (bar >= sh->vec_empty && bar < sh->vec_empty + 4) ? 8 : bar == &sh->acc_empty ? 4
+                   : bar >= sh->item_empty && bar < sh->item_empty + kItems ? 15 : 1);
   }
   if (threadIdx.x == 0) sh->abort_flag = sh->bad = 0;
   fence_barrier_init();
@@ -235,132 +237,97 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
         }
       }
     } else if (warp == 1) {
-      // ---------------------------------------------------------------- MMA issuer
+      // ---------------------------------------------------------------- S and dP
       const uint32_t el = elect_one();
       const uint32_t fmt = BF16 ? 1u : 0u;
       const uint32_t hi_sw = smem_desc_hi(1024, true);
-      const uint64_t x_d = smem_desc_from(smem_u32(x_smem), 16, hi_sw), y_d = smem_desc_from(smem_u32(y_smem), 16, hi_sw),
-                     ymn_d = smem_desc_from(smem_u32(y_smem), kY, hi_sw);
-      const uint32_t id_qk = instr_desc(fmt, 128, XC * 64, 0, 1), id_v = instr_desc(fmt, 128, VC * 64, 0, 1);
+      const uint64_t x_d = smem_desc_from(smem_u32(x_smem), 16, hi_sw), y_d = smem_desc_from(smem_u32(y_smem), 16, hi_sw);
       int st = 0, y_par = 0, xb = 0, x_par = 0, buf = 0;
-      uint32_t ds_par = 0, acc_par = 1;
-      // (stage and score buffer of the block whose products come next: st, buf)
-      auto scores = [&](int stage, int b2, uint32_t cols) {
-        const uint32_t id = instr_desc(fmt, 128, cols, 0, 0);
-        const uint64_t xd = x_d + (uint64_t)(xb * (kX >> 4)), yd = y_d + (uint64_t)(stage * (kYStage >> 4));
-#pragma unroll
-        for (int k = 0; k < 4 * XC; ++k)
-          umma_ss_el(el, tmem + b2 * N, xd + (k >> 2) * (kChunk >> 4) + 2 * (k & 3), yd + (k >> 2) * (kY >> 4) + 2 * (k & 3), id, k ? 1u : 0u);
-        umma_commit_el(el, &sh->s_full[b2]);
-      };
-      auto dprods = [&](int stage, uint32_t cols) {
-        const uint32_t id = instr_desc(fmt, 128, cols, 0, 0);
-        const uint64_t xd = x_d + (uint64_t)((xb * kX + XC * kChunk) >> 4), yd = y_d + (uint64_t)((stage * kYStage + XC * kY) >> 4);
-#pragma unroll
-        for (int k = 0; k < 4 * VC; ++k)
-          umma_ss_el(el, tmem + S::kDP, xd + (k >> 2) * (kChunk >> 4) + 2 * (k & 3), yd + (k >> 2) * (kY >> 4) + 2 * (k & 3), id, k ? 1u : 0u);
-        umma_commit_el(el, &sh->dp_full);
-      };
+      uint32_t ds_par = 0, sd_par = 3;                           // sd_par: a bit per score buffer
+      bool open = false;                                         // a block whose dP has not been read yet
       BwdItem w;
       while (take(w)) {
         if (!w.nb) continue;
         wait(&sh->x_full[xb], x_par);
-        wait(&sh->y_full[st], y_par);
-        if (!ok) break;
-        tc_fence_after();
-        Walk y(w, a.G);
-        uint32_t cols = y.cols(a.ns);
-        scores(st, buf, cols);
-        dprods(st, cols);
-        if (w.nb == 1) umma_commit_el(el, &sh->x_empty[xb]);
-        for (int n = 0; n < w.nb; ++n) {
-          const bool more = n + 1 < w.nb;
-          int st2 = st + 1, par2 = y_par;
-          if (st2 == p.stages) { st2 = 0; par2 ^= 1; }
-          y.next(w);
-          const uint32_t cols2 = more ? y.cols(a.ns) : 0;
-          if (more) {
-            wait(&sh->y_full[st2], par2);
-            if (!ok) break;
-            tc_fence_after();
-            scores(st2, buf ^ 1, cols2);
-          }
-          wait(&sh->ds_ready, ds_par);
-          ds_par ^= 1;
+        const uint64_t xq = x_d + (uint64_t)(xb * (kX >> 4)), xv = xq + (XC * kChunk >> 4);
+        for (Walk y(w, a.G); ok && y.n < w.nb; y.next(w)) {
+          const uint32_t id = instr_desc(fmt, 128, y.cols(a.ns), 0, 0);
+          const uint64_t yq = y_d + (uint64_t)(st * (kYStage >> 4)), yv = yq + (XC * kY >> 4);
+          wait(&sh->y_full[st], y_par);
+          wait(&sh->s_done[buf], sd_par >> buf & 1u);            // the products have read the P and dS over the scores before the last
+          sd_par ^= 1u << buf;
           if (!ok) break;
           tc_fence_after();
-          if (more) {
-            dprods(st2, cols2);
-            if (n + 2 == w.nb) umma_commit_el(el, &sh->x_empty[xb]);
-          }
-          if (n == 0) {
-            wait(&sh->acc_empty, acc_par);
-            acc_par ^= 1;
+#pragma unroll
+          for (int k = 0; k < 4 * XC; ++k)
+            umma_ss_el(el, tmem + buf * N, xq + (k >> 2) * (kChunk >> 4) + 2 * (k & 3), yq + (k >> 2) * (kY >> 4) + 2 * (k & 3), id, k ? 1u : 0u);
+          umma_commit_el(el, &sh->s_full[buf]);
+          if (open) {                                            // the groups have read the dP before
+            wait(&sh->ds_ready[buf ^ 1], ds_par >> (buf ^ 1) & 1u);
+            ds_par ^= 1u << (buf ^ 1);
             if (!ok) break;
             tc_fence_after();
           }
+          open = true;
+#pragma unroll
+          for (int k = 0; k < 4 * VC; ++k)
+            umma_ss_el(el, tmem + S::kDP, xv + (k >> 2) * (kChunk >> 4) + 2 * (k & 3), yv + (k >> 2) * (kY >> 4) + 2 * (k & 3), id, k ? 1u : 0u);
+          umma_commit_el(el, &sh->dp_full);
+          buf ^= 1;
+          if (++st == p.stages) { st = 0; y_par ^= 1; }
+        }
+        if (!ok) break;
+        umma_commit_el(el, &sh->x_empty[xb]);
+        if (++xb == p.xbufs) { xb = 0; x_par ^= 1; }
+      }
+    } else if (warp == 3) {
+      // ---------------------------------------------------------------- dQ += dS K, or dV += P dO and dK += dS Q
+      const uint32_t el = elect_one();
+      const uint32_t fmt = BF16 ? 1u : 0u;
+      const uint64_t y_d = smem_desc_from(smem_u32(y_smem), kY, smem_desc_hi(1024, true));
+      const uint32_t id_qk = instr_desc(fmt, 128, XC * 64, 0, 1), id_v = instr_desc(fmt, 128, VC * 64, 0, 1);
+      int st = 0, buf = 0;
+      uint32_t ds_par = 0, acc_par = 1;
+      BwdItem w;
+      while (take(w)) {
+        if (!w.nb) continue;
+        wait(&sh->acc_empty, acc_par);                           // the accumulators of the item before have been read
+        acc_par ^= 1;
+        for (Walk y(w, a.G); ok && y.n < w.nb; y.next(w)) {
+          const uint32_t s_tm = tmem + buf * N, acc = y.n ? 1u : 0u;
+          const uint64_t yq = y_d + (uint64_t)(st * (kYStage >> 4)), yv = yq + (XC * kY >> 4);
+          wait(&sh->ds_ready[buf], ds_par >> buf & 1u);
+          ds_par ^= 1u << buf;
+          if (!ok) break;
+          tc_fence_after();
           // a chunk of 16 columns holds 16 P (KIND 2) and 16 dS, packed into 8 columns each
-          const uint32_t s_tm = tmem + buf * N, acc = n ? 1u : 0u;
-          const uint64_t yq = ymn_d + (uint64_t)((st * kYStage) >> 4), yv = yq + (XC * kY >> 4);
           if constexpr (KIND == 2) {
 #pragma unroll
             for (int k = 0; k < N / 16; ++k) umma_ts_el(el, tmem + S::kAccV, s_tm + 16 * k, yv + 128 * k, id_v, k ? 1u : acc);
 #pragma unroll
             for (int k = 0; k < N / 16; ++k) umma_ts_el(el, tmem + S::kAccQK, s_tm + 16 * k + 8, yq + 128 * k, id_qk, k ? 1u : acc);
-          } else if (cols == N) {
+          } else if (y.window()) {
 #pragma unroll
             for (int k = 0; k < N / 16; ++k) umma_ts_el(el, tmem + S::kAccQK, s_tm + 16 * k, yq + 128 * k, id_qk, k ? 1u : acc);
           } else {
-            for (uint32_t k = 0; k < cols / 16; ++k) umma_ts_el(el, tmem + S::kAccQK, s_tm + 16 * k, yq + 128 * k, id_qk, k ? 1u : acc);
+            const int steps = y.cols(a.ns) >> 4;
+            for (int k = 0; k < steps; ++k) umma_ts_el(el, tmem + S::kAccQK, s_tm + 16 * k, yq + 128 * k, id_qk, k ? 1u : acc);
           }
+          umma_commit_el(el, &sh->s_done[buf]);
           umma_commit_el(el, &sh->y_empty[st]);
-          cols = cols2;
-          st = st2;
-          y_par = par2;
           buf ^= 1;
+          if (++st == p.stages) st = 0;
         }
         if (!ok) break;
         umma_commit_el(el, &sh->acc_full);
-        if (++xb == p.xbufs) { xb = 0; x_par ^= 1; }
       }
-    } else if (KIND == 2 && warp == 2) {
-      // ---------------------------------------------------------------- softmax statistics of the streamed rows
-      int v = 0, par = 1;
-      BwdItem w;
-      while (take(w)) {
-        if (!w.nb) continue;
-        for (Walk y(w, a.G); y.n < w.nb; y.next(w)) {
-          const int row = y.y0;
-          const int64_t at = ((int64_t)w.b * a.Hq + y.h) * a.N + row;
-          float l[4], d[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int r = lane + 32 * x;
-            const bool in = r < N && row + r < w.len;
-            l[x] = in ? a.lse[at + r] : INFINITY;                 // a row behind the end: P = exp2(-inf)
-            d[x] = in ? a.delta[at + r] : 0.f;
-          }
-          wait(&sh->vec_empty[v], par);
-          if (!ok) break;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            sh->vec[v][0][lane + 32 * x] = -l[x];
-            sh->vec[v][1][lane + 32 * x] = -d[x];
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh->vec_full[v]);
-          if (++v == 4) { v = 0; par ^= 1; }
-        }
-        if (!ok) break;
-      }
-    } else if (warp == 3) {
-      // ---------------------------------------------------------------- items
-      int s = 0, par = 1;
-      for (int item = blockIdx.x; ok; item += gridDim.x) {
-        const bool end = item >= p.n_items;
-        BwdItem w;
+    } else if (warp == 2) {
+      // ---------------------------------------------------------------- items and softmax statistics
+      int s = 0, par = 1, item = blockIdx.x, v = 0, v_par = 1;
+      // the next item into the ring, with the end mark after the last; false once it is in, or a wait gave up
+      auto hand_out = [&](BwdItem& w) {
         w.nb = -1;
-        if (!end) w = bwd_item<KIND, N>(p, item);
+        if (item < p.n_items) w = bwd_item<KIND, N>(p, item);
         float l[4], d[4];
         if (KIND == 1 && w.nb > 0) {
           const int64_t at = ((int64_t)w.b * a.Hq + w.h) * a.N + w.x0;
@@ -372,7 +339,7 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
           }
         }
         wait(&sh->item_empty[s], par);
-        if (!ok) break;
+        if (!ok) return false;
         if (KIND == 1 && w.nb > 0) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -383,8 +350,42 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
         if (lane == 0) sh->item[s] = w;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->item_full[s]);
-        if (end) break;
         if (++s == kItems) { s = 0; par ^= 1; }
+        item += gridDim.x;
+        return w.nb >= 0;
+      };
+      BwdItem w, next;
+      bool more = hand_out(w);
+      // KIND 2: one item ahead of the one whose blocks' statistics are written
+      while (KIND == 1 && more) more = hand_out(w);
+      while (KIND == 2 && more) {
+        more = hand_out(next);
+        if (!ok) break;
+        if (w.nb)
+          for (Walk y(w, a.G); y.n < w.nb; y.next(w)) {
+            const int row = y.y0;
+            const int64_t at = ((int64_t)w.b * a.Hq + y.h) * a.N + row;
+            float l[4], d[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int r = lane + 32 * x;
+              const bool in = r < N && row + r < w.len;
+              l[x] = in ? a.lse[at + r] : INFINITY;               // a row behind the end: P = exp2(-inf)
+              d[x] = in ? a.delta[at + r] : 0.f;
+            }
+            wait(&sh->vec_empty[v], v_par);
+            if (!ok) break;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              sh->vec[v][0][lane + 32 * x] = -l[x];
+              sh->vec[v][1][lane + 32 * x] = -d[x];
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->vec_full[v]);
+            if (++v == 4) { v = 0; v_par ^= 1; }
+          }
+        if (!ok) break;
+        w = next;
       }
     }
   } else if (warp < 12) {
@@ -516,7 +517,7 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&sh->ds_ready);
+          mbar_arrive(&sh->ds_ready[buf]);
           if constexpr (KIND == 2) mbar_arrive(&sh->vec_empty[v]);
         }
         buf ^= 1;
