@@ -56,7 +56,7 @@ int check_axes(const rope_axes_t* r, int32_t C) {
 int check_heads(int32_t B, int32_t Hq, int32_t Hkv) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0) return fail(E_SHAPE, "batch and heads must be positive");
   if (Hq % Hkv) return fail(E_SHAPE, "query heads (%d) must be a multiple of key heads (%d)", Hq, Hkv);
-  if (B > 65535 || Hq > 65535) return fail(E_SHAPE, "batch and heads must be at most 65535");
+  if (B > 65535 || Hq > 65535 || Hkv > 8191) return fail(E_SHAPE, "batch and query heads must be at most 65535, key heads at most 8191");
   return 0;
 }
 
@@ -173,7 +173,7 @@ int launch_f32(const swa::sink::Args& a, float* part, cudaStream_t st) {
   if (KIND != 2 || p.pieces <= 1) return 0;
   constexpr int R = swa::sink::kF32Rows, WARPS = swa::sink::kRowWarps;
   const swa::sink::JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, R, R, a.dqk + a.dv_dim, 4, part};
-  e = swa::launch_pdl(swa::sink::join_kernel<float>, dim3(std::min(p.n_sb * R, a.N + WARPS - 1) / WARPS, a.Hkv, a.B), 32 * WARPS, 0, st, jp);
+  e = swa::launch_pdl(swa::sink::join_kernel<float>, dim3(std::min(p.n_sb * R, a.N + WARPS - 1) / WARPS, a.Hkv * 8, a.B), 32 * WARPS, 0, st, jp);
   return launched(e, "sink join");
 }
 

@@ -210,47 +210,57 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
 // rows into pieces of piece_len, each of which leaves its sums in part [B, Hkv, n_sb, pieces, rows * (d_qk + d_v)], row j and column c of
 // them at j * s_row + c / 4 * s_col4 + c % 4.  Added here in the order of the pieces, one warp per row; a block that is a single piece
 // has gone straight out.
+// Whether `nb` blocks of the stream from `first` on hold one that rows other than sinks can see: the first `near` of a head's `per_head`.  The
+// other pieces leave sums for the sinks' rows only.
+__device__ __forceinline__ bool piece_near(int first, int nb, int per_head, int near) {
+  const int at = first % per_head;
+  return at < near || at + nb > per_head;
+}
+
 struct JoinParams {
   Args a;
   int n_sb, pieces, piece_len, rows, stream, s_row, s_col4;
   const float* part;
 };
 
+// grid = (rows / 8, Hkv * 8, B): a warp has one row and 32 of its columns (with a warp for all of a row's columns 16384 tokens' 14 pieces took 17 us).
 template <typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) join_kernel(const __grid_constant__ JoinParams p) {
   __shared__ float smem[kRowWarps][2 * kMaxDim];
   pdl_enter();
   pdl_wait();
   const Args& a = p.a;
-  const int lane = threadIdx.x & 31, j = blockIdx.x * kRowWarps + (threadIdx.x >> 5), hk = blockIdx.y, b = blockIdx.z;
-  const int len = seq_len(a, b), blk = j / p.rows, x0 = blk * p.rows;
-  if (j >= a.N || blk >= p.n_sb || x0 >= len) return;            // (a block behind the end: zeros, written by its first piece)
+  const int lane = threadIdx.x & 31, j = blockIdx.x * kRowWarps + (threadIdx.x >> 5), hk = blockIdx.y >> 3, c = 32 * (blockIdx.y & 7) + lane, b = blockIdx.z;
+  const int len = seq_len(a, b), blk = j / p.rows, x0 = blk * p.rows, d = a.dqk + a.dv_dim;
+  if (j >= a.N || blk >= p.n_sb || x0 >= len || c - lane >= d) return;            // (a block behind the end: zeros, written by its first piece)
   const int all = (len - x0 + p.stream - 1) / p.stream * a.G;
   if (all <= p.piece_len) return;
-  const int pieces = (all + p.piece_len - 1) / p.piece_len, d = a.dqk + a.dv_dim;
-  const float* part = p.part + (((int64_t)b * a.Hkv + hk) * p.n_sb + blk) * p.pieces * (int64_t)p.rows * d + (j - x0) * p.s_row + (lane >> 2) * p.s_col4 + (lane & 3);
-  float acc[8] = {};
-#pragma unroll 4
-  for (int x = 0; x < (j < len ? pieces : 0); ++x) {
+  const int pieces = j < len ? (all + p.piece_len - 1) / p.piece_len : 0, per_head = all / a.G, near = p.piece_len / a.G;
+  const bool sink = j < a.ns;
+  const int64_t step = (int64_t)p.rows * d;
+  const float* part = p.part + (((int64_t)b * a.Hkv + hk) * p.n_sb + blk) * p.pieces * step + (j - x0) * p.s_row + (c >> 2) * p.s_col4 + (c & 3);
+  float acc = 0.f;
+  for (int p0 = 0; p0 < pieces; p0 += 32) {
+    const int mine = p0 + lane;
+    uint32_t has = __ballot_sync(0xffffffffu, mine < pieces && (sink || piece_near(mine * p.piece_len, min(p.piece_len, all - mine * p.piece_len), per_head, near)));
+    if (c >= d) has = 0;
+    const float* from = part + p0 * step;
+#pragma unroll 1
+    for (int x = 0; has >> x; x += 8, from += 8 * step) {
+      float v[8];                                                // eight pieces in flight
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
-      if (lane + 32 * t < d) acc[t] += part[(int64_t)x * p.rows * d + 8 * t * p.s_col4];
+      for (int e = 0; e < 8; ++e) v[e] = has >> x >> e & 1u ? from[e * step] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc += v[e];
+      if (x == 24) break;
+    }
   }
-  bool bad = false;
-#pragma unroll
-  for (int t = 0; t < 8; ++t) bad |= lane + 32 * t < d && !(fabsf(acc[t]) <= 3.0e38f);
-  if (__any_sync(0xffffffffu, bad)) {
+  if (__any_sync(0xffffffffu, c < d && !(fabsf(acc) <= 3.0e38f))) {               // the whole row again (the row's other warps may do the same)
     row_dkdv<T>(a, b, hk, j, smem[threadIdx.x >> 5]);
     return;
   }
-  T* k = (T*)a.dk.ptr + b * a.dk.s0 + hk * a.dk.s1 + (int64_t)j * a.dk.s2;
-  T* v = (T*)a.dv.ptr + b * a.dv.s0 + hk * a.dv.s1 + (int64_t)j * a.dv.s2;
-#pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    const int c = lane + 32 * t;
-    if (c < a.dqk) k[c * a.dk.s3] = from_f<T>(acc[t] * a.scale);
-    else if (c < d) v[(c - a.dqk) * a.dv.s3] = from_f<T>(acc[t]);
-  }
+  if (c < a.dqk) ((T*)a.dk.ptr)[b * a.dk.s0 + hk * a.dk.s1 + (int64_t)j * a.dk.s2 + c * a.dk.s3] = from_f<T>(acc * a.scale);
+  else if (c < d) ((T*)a.dv.ptr)[b * a.dv.s0 + hk * a.dv.s1 + (int64_t)j * a.dv.s2 + (c - a.dqk) * a.dv.s3] = from_f<T>(acc);
 }
 
 }  // namespace sink

@@ -146,7 +146,7 @@ int launch_bwd(const Args& a, int dtype, void* scratch, int32_t* status, cudaStr
   cudaError_t e = allow_smem((const void*)kern);
   if (e == cudaSuccess) e = launch_pdl(kern, dim3(std::min(p.n_items, tc::sm_count())), kThreads, smem, st, txq, txv, tyq, tyv, toq, tov, p);
   if (e == cudaSuccess && KIND == 2 && p.pieces > 1) {
-    const dim3 grid(std::min(p.n_sb * kTile, a.N + kRowWarps - 1) / kRowWarps, a.Hkv, a.B);
+    const dim3 grid(std::min(p.n_sb * kTile, a.N + kRowWarps - 1) / kRowWarps, a.Hkv * 8, a.B);
     const JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, kTile, N, 4, 4 * kTile, p.part};
     e = dtype == SWA_BF16 ? launch_pdl(join_kernel<__nv_bfloat16>, grid, 32 * kRowWarps, 0, st, jp)
                           : launch_pdl(join_kernel<__half>, grid, 32 * kRowWarps, 0, st, jp);

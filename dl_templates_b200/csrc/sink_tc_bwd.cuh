@@ -242,6 +242,7 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
       const uint32_t fmt = BF16 ? 1u : 0u;
       const uint32_t hi_sw = smem_desc_hi(1024, true);
       const uint64_t x_d = smem_desc_from(smem_u32(x_smem), 16, hi_sw), y_d = smem_desc_from(smem_u32(y_smem), 16, hi_sw);
+      const int kq = steps16(a.dqk), kv = steps16(a.dv_dim);
       int st = 0, y_par = 0, xb = 0, x_par = 0, buf = 0;
       uint32_t ds_par = 0, sd_par = 3;                           // sd_par: a bit per score buffer
       bool open = false;                                         // a block whose dP has not been read yet
@@ -258,9 +259,7 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
           sd_par ^= 1u << buf;
           if (!ok) break;
           tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < 4 * XC; ++k)
-            umma_ss_el(el, tmem + buf * N, xq + (k >> 2) * (kChunk >> 4) + 2 * (k & 3), yq + (k >> 2) * (kY >> 4) + 2 * (k & 3), id, k ? 1u : 0u);
+          scores_mma<XC>(el, tmem + buf * N, xq, yq, kChunk >> 4, kY >> 4, id, kq);
           umma_commit_el(el, &sh->s_full[buf]);
           if (open) {                                            // the groups have read the dP before
             wait(&sh->ds_ready[buf ^ 1], ds_par >> (buf ^ 1) & 1u);
@@ -269,9 +268,7 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
             tc_fence_after();
           }
           open = true;
-#pragma unroll
-          for (int k = 0; k < 4 * VC; ++k)
-            umma_ss_el(el, tmem + S::kDP, xv + (k >> 2) * (kChunk >> 4) + 2 * (k & 3), yv + (k >> 2) * (kY >> 4) + 2 * (k & 3), id, k ? 1u : 0u);
+          scores_mma<VC>(el, tmem + S::kDP, xv, yv, kChunk >> 4, kY >> 4, id, kv);
           umma_commit_el(el, &sh->dp_full);
           buf ^= 1;
           if (++st == p.stages) { st = 0; y_par ^= 1; }
@@ -285,7 +282,7 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
       const uint32_t el = elect_one();
       const uint32_t fmt = BF16 ? 1u : 0u;
       const uint64_t y_d = smem_desc_from(smem_u32(y_smem), kY, smem_desc_hi(1024, true));
-      const uint32_t id_qk = instr_desc(fmt, 128, XC * 64, 0, 1), id_v = instr_desc(fmt, 128, VC * 64, 0, 1);
+      const uint32_t id_qk = instr_desc(fmt, 128, 16 * steps16(a.dqk), 0, 1), id_v = instr_desc(fmt, 128, 16 * steps16(a.dv_dim), 0, 1);
       int st = 0, buf = 0;
       uint32_t ds_par = 0, acc_par = 1;
       BwdItem w;
@@ -547,6 +544,7 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
       if (!ok) break;
       tc_fence_after();
       const bool live = w.x0 + r < w.len;
+      const bool counts = KIND == 2 && w.piece >= 0 && (w.x0 + r < a.ns || piece_near(w.first, w.nb, w.per_head, p.piece_len / a.G));
       uint64_t z = 0ull;
       // accumulators, 32 columns at a time: dV, then dQ or dK
       constexpr int kV = KIND == 2 ? 2 * VC : 0, kAll = kV + 2 * XC;
@@ -569,10 +567,10 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
                         (int64_t)((is_v ? a.dqk : 0) + col) * kTile + r * 4;
 #pragma unroll
           for (int u = 0; u < 8; ++u)
-            if (col + 4 * u < (is_v ? a.dv_dim : a.dqk))
+            if (counts && col + 4 * u < (is_v ? a.dv_dim : a.dqk))
               *reinterpret_cast<uint4*>(part + u * 4 * kTile) = make_uint4(q[4 * u], q[4 * u + 1], q[4 * u + 2], q[4 * u + 3]);
         } else if (row0 < a.N) {
-          store_columns<BF16>(q, is_v ? 1.f : a.scale, live, z, stg, lane, is_v ? &tm_ov : &tm_oqk, col, row0, w.h, w.b);
+          store_columns<BF16>(q, is_v ? 1.f : a.scale, live, z, stg, lane, is_v ? &tm_ov : &tm_oqk, col, is_v ? a.dv_dim : a.dqk, row0, w.h, w.b);
         }
       }
       if (live && has_nan(z)) sh->bad = 1;

@@ -28,11 +28,12 @@ __device__ __forceinline__ uint32_t below(int n, int w) {
   return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
 }
 
-// 32 columns of an accumulator: this thread's row, times f, as 16-bit values through the warp's staging buffer to rows row0 .. row0 + 31
-// of the output; `z` becomes a NaN with any infinity or NaN.  The warp's lanes together; `keep`: the row counts, else zeros.
+// 32 columns of an accumulator, from column `col` of d on: this thread's row, times f, as 16-bit values through the warp's staging buffer to
+// rows row0 .. row0 + 31 of the output; `z` becomes a NaN with any infinity or NaN.  The warp's lanes together; `keep`: the row
+// counts, else zeros.  (Columns from d on have never been written.)
 template <bool BF16>
 __device__ __forceinline__ void store_columns(const uint32_t* x, float f, bool keep, uint64_t& z, uint8_t* stg, int lane, const CUtensorMap* map,
-                                              int col, int row0, int h, int b) {
+                                              int col, int d, int row0, int h, int b) {
   using namespace ptx;
   const uint64_t f2 = f2_pack(f, f);
   const uint32_t row = smem_u32(stg) + lane * 64, sw = (uint32_t)(lane >> 1 & 3) << 4;
@@ -41,6 +42,7 @@ __device__ __forceinline__ void store_columns(const uint32_t* x, float f, bool k
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     uint32_t w[4];
+    if (col + 8 * u >= d) break;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint64_t y = f2_mul(f2_pack(__uint_as_float(x[8 * u + 2 * e]), __uint_as_float(x[8 * u + 2 * e + 1])), f2);
@@ -66,7 +68,24 @@ __device__ __forceinline__ void store_zeros(uint8_t* stg, int lane, const CUtens
 #pragma unroll
   for (int e = 0; e < 32; ++e) x[e] = 0u;
   uint64_t z = 0ull;
-  for (int c = 0; c < d; c += 32) store_columns<BF16>(x, 0.f, false, z, stg, lane, map, c, row0, h, b);
+  for (int c = 0; c < d; c += 32) store_columns<BF16>(x, 0.f, false, z, stg, lane, map, c, d, row0, h, b);
+}
+
+// Steps of 16 elements of a contraction over a head dim, and the columns of an accumulator of that many: heads that fill no chunk of 64
+// pay for what they have (d = 80 as 128: 63 % more of every product).
+__device__ __forceinline__ int steps16(int d) { return (d + 15) >> 4; }
+
+// D = A B^T over `steps` steps of 16 elements of chunks of 64, `a16` and `b16` bytes / 16 apart; a whole number of chunks without a test
+// per step (with one, the products of d = 128 waited for their issue: 8 % of the forward kernel).
+template <int CHUNKS>
+__device__ __forceinline__ void scores_mma(uint32_t el, uint32_t d_tm, uint64_t ad, uint64_t bd, uint32_t a16, uint32_t b16, uint32_t id, int steps) {
+  if (steps == 4 * CHUNKS) {
+#pragma unroll
+    for (int k = 0; k < 4 * CHUNKS; ++k) ptx::umma_ss_el(el, d_tm, ad + (k >> 2) * a16 + 2 * (k & 3), bd + (k >> 2) * b16 + 2 * (k & 3), id, k ? 1u : 0u);
+  } else {
+#pragma unroll 1
+    for (int k = 0; k < steps; ++k) ptx::umma_ss_el(el, d_tm, ad + (k >> 2) * a16 + 2 * (k & 3), bd + (k >> 2) * b16 + 2 * (k & 3), id, k ? 1u : 0u);
+  }
 }
 
 __device__ __forceinline__ bool has_nan(uint64_t z) {

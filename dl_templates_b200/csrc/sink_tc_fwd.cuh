@@ -192,6 +192,7 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const uint32_t hi_sw = smem_desc_hi(1024, true);
       const uint64_t q_d = smem_desc_from(smem_u32(q_smem), 16, hi_sw), k_d = smem_desc_from(smem_u32(k_smem), 16, hi_sw);
       const uint32_t id_full = instr_desc(fmt, 128, N, 0, 0);
+      const int kq = steps16(a.dqk);
       int ks = 0, kpar = 0, q_par = 0;
       uint32_t sf_par = 3;                                       // a bit per tile
       FwdItem w;
@@ -213,9 +214,7 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             tc_fence_after();
             const uint32_t id = blk >= w.lo[t] ? id_full : instr_desc(fmt, 128, fwd_cols<N>(a, blk, w.lo[t]), 0, 0);
             const uint64_t qd = q_d + (uint64_t)(t * QC * (kChunk >> 4));
-#pragma unroll
-            for (int k = 0; k < 4 * QC; ++k)
-              umma_ss_el(el, tmem + t * N, qd + (k >> 2) * (kChunk >> 4) + 2 * (k & 3), kd + (k >> 2) * (kB >> 4) + 2 * (k & 3), id, k ? 1u : 0u);
+            scores_mma<QC>(el, tmem + t * N, qd, kd, kChunk >> 4, kB >> 4, id, kq);
             umma_commit_el(el, &sh->s_full[t]);
           }
           if (!ok) break;
@@ -228,7 +227,7 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     } else if (warp == 3) {
       // ---------------------------------------------------------------- O_t += P_t V
       const uint32_t el = elect_one();
-      const uint32_t id_pv = instr_desc(BF16 ? 1u : 0u, 128, kOCols, 0, 1);
+      const uint32_t id_pv = instr_desc(BF16 ? 1u : 0u, 128, 16 * steps16(a.dv_dim), 0, 1);
       const uint64_t v_d = smem_desc_from(smem_u32(v_smem), kB, smem_desc_hi(1024, true));
       int vs = 0, vpar = 0;
       uint32_t p_par = 0, o_par = 3;                             // a bit per tile
@@ -498,7 +497,7 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               mbar_arrive(&sh->l_empty[t]);
             }
           }
-          if (row0 < a.N && c < a.dv_dim) store_columns<BF16>(x, inv, live, z, stg, lane, &tm_o, c, row0, w.h[t], w.b);
+          if (row0 < a.N && c < a.dv_dim) store_columns<BF16>(x, inv, live, z, stg, lane, &tm_o, c, a.dv_dim, row0, w.h[t], w.b);
         }
         if (live && has_nan(z)) sh->bad = 1;
       }
