@@ -54,9 +54,13 @@ const char* tc_unsupported(const sink_geom_t* g, const swa_tensor_t* const* ts, 
   if (g->d_qk % 8 || g->d_v % 8 || g->d_qk > 128 || g->d_v > 128) return "head dims must be multiples of 8 up to 128";
   if (!(g->sm_scale > 0.f)) return "sm_scale must be positive";
   if ((int64_t)((g->N + kTile - 1) / kTile) * g->B * g->Hq > (1 << 30)) return "too many tiles";
-  for (int i = 0; ts && i < n; ++i) {
+  // The kernels' waits last about a second: a dK/dV tile's stream of G window rows has to end well before (a block of 64 to 128 takes a
+  // microsecond).
+  if ((int64_t)(g->Hq / g->Hkv) * (g->window < g->N ? g->window : g->N) > (1 << 25)) return "query heads per key head times window is above 2^25";
+  for (int i = 0; ts && i < n; ++i) {                            // q, k, v, o[, do, dq, dk, dv]
     const int64_t* s = ts[i]->stride;
-    const int64_t extent[3] = {g->B, 2, g->N};                   // (heads: of q or of k; a stride of 0 is refused for either)
+    const bool of_k = i == 1 || i == 2 || i >= 6;
+    const int64_t extent[3] = {g->B, of_k ? g->Hkv : g->Hq, g->N};
     if (s[3] != 1 || (uintptr_t)ts[i]->ptr % 16) return "rows must be contiguous and start on 16-byte boundaries";
     for (int d = 0; d < 3; ++d)
       if (extent[d] > 1 && (s[d] <= 0 || s[d] % 8 || s[d] >= (int64_t)1 << 38)) return "strides must be positive multiples of 8";

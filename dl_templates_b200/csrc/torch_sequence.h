@@ -29,6 +29,9 @@ void check_writable(const Tensor& t, const char* name) {
 // While a graph is captured, autograd's engine would record events on the stream that an older graph's leaf accumulators live on,
 // which is not part of the capture; what follows ends the process inside the engine.  Refused here, while nothing has been launched.
 void check_capture(std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    if (!t->is_cuda()) return;                                   // (refused further on)
+  const c10::cuda::OptionalCUDAGuard guard((*inputs.begin())->device());
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
   for (const Tensor* t : inputs) {
     if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;

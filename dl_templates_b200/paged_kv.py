@@ -10,7 +10,8 @@ both calls of a step.  All three live on the device and are read there: a step c
 while they change.  A page number outside the cache is no page -- nothing is written to it and nothing of it is seen -- so that
 pages that neither the window nor the sinks reach can be given back and their entries set to -1.
 
-Neither call records gradients.
+Two new tokens of one call never share a slot: the pages they fall into belong to one sequence each (a page that several sequences
+read, a shared prefix, may stand in all their tables).  Neither call records gradients.
 """
 from __future__ import annotations
 

@@ -374,6 +374,50 @@ def test_cache_calls_refuse():
             bad()
 
 
+def test_offsets_beyond_32_bits():
+    """A cache and query tensors of more than 2^31 elements: what lies behind is what a small tensor of the same rows gives."""
+    g = gen(21)
+    Hkv, page, d, n = 8, 64, 128, 300
+    n_pages = (1 << 31) // (Hkv * page * d) + 8
+    kc, vc = (torch.zeros(n_pages, Hkv, page, d, dtype=BF, device=DEV) for _ in range(2))
+    k, v, q = randn(g, 1, Hkv, n, d).to(DEV), randn(g, 1, Hkv, n, d).to(DEV), randn(g, 1, 16, 1, d).to(DEV)
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    outs = []
+    for cache, first in (((kc, vc), n_pages - 5), ((kc[:5].clone(), vc[:5].clone()), 0)):
+        table = torch.arange(first, first + 5, dtype=torch.int32, device=DEV)[None]
+        swa.kv_append_rope(None, k, v, None, None, *cache, table, lens)
+        outs.append(swa.sink_swa_decode(q, *cache, table, lens, 200, 4, 0.1))
+        assert torch.equal(cache[0][first:first + 4].transpose(0, 1).reshape(Hkv, -1, d), k[0, :, :256])
+    assert torch.equal(*outs)
+    del kc, vc, cache
+    N, H = 1 << 17, 129                               # 129 heads of 2^24 elements
+    q, do = (torch.zeros(1, H, N, d, dtype=BF, device=DEV) for _ in range(2))
+    k, v = randn(g, 1, 1, N, d).to(DEV), randn(g, 1, 1, N, d).to(DEV)
+    q[:, -1], do[:, -1] = randn(g, N, d).to(DEV), randn(g, N, d).to(DEV)
+    o, lse = swa.sink_swa_forward(q, k, v, 60, 3, 0.1)
+    o1, lse1 = swa.sink_swa_forward(q[:, -1:], k, v, 60, 3, 0.1)
+    assert torch.equal(o[:, -1:], o1) and torch.equal(lse[:, -1:], lse1)
+    dq, dk, dv = swa.sink_swa_backward(q, k, v, o, lse, do, 60, 3, 0.1)
+    dq1, dk1, dv1 = swa.sink_swa_backward(q[:, -1:], k, v, o1, lse1, do[:, -1:], 60, 3, 0.1)
+    # the other heads' dO is zero, and so is their dS (the block with the sinks is summed in other pieces, so in another order)
+    assert torch.equal(dq[:, -1:], dq1) and torch.equal(dv[:, :, 128:], dv1[:, :, 128:]) and torch.equal(dk[:, :, 128:], dk1[:, :, 128:])
+    assert bool(torch.isfinite(dk.float()).all()) and bool(torch.isfinite(dv.float()).all())
+    x = swa.rope_axes_apply_to(q, torch.zeros(1, N, dtype=torch.int32, device=DEV), (swa.make_cs_table(64, 4, device=DEV),))
+    assert torch.equal(x[:, -1], q[:, -1])
+    swa.check_status()
+
+
+def test_largest_sinks_and_one_token_windows():
+    """1024 sinks over many blocks, windows of one token, more heads than one MMA tile of the decoding kernel has."""
+    for case in ((1, 2, 1, 1500, 1, 1024, 64, 64, None), (1, 24, 1, 260, 33, 2, 64, 64, [259])):
+        _, _, _, _, W, ns, _, _, lens = case
+        t, scale = attn_case(case, BF)
+        want, bound = orc.attention(t["q"], t["k"], t["v"], lens, W, ns, scale, t["do"])
+        got = run_attn(t, lens_tensor(lens), W, ns, scale)
+        for n in want:
+            orc.check(got[n], want[n], bound[n], n)
+
+
 # ---- together -----------------------------------------------------------------------------------------------------------------
 def test_prompt_and_steps_agree_with_the_whole_sequence():
     """Rotate and attend over a prompt, put it into the cache, then single steps captured into a CUDA graph and replayed: the steps' results are

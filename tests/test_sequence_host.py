@@ -121,6 +121,13 @@ def test_surface_takes_what_it_documents():
 
 def test_selection_rule():
     q = torch.zeros(1, 4, 8, 64, dtype=BF)
+    assert swa.sink_selected_impl(q, q, q, 4, 1) == "tc"
+    for kw, impl in ((dict(d_qk=72, d_v=8), 2), (dict(d_qk=20), 1), (dict(d_qk=136), 1), (dict(dtype=0), 1), (dict(sm_scale=0.0), 1), (dict(sm_scale=-1.0), 1),
+                     (dict(impl=1), 1), (dict(Hq=64, Hkv=1, N=1 << 20, window=1 << 20), 1), (dict(Hq=32, Hkv=1, N=1 << 20, window=1 << 20), 2)):
+        g = geom(**kw)
+        assert LIB.sink_swa_select(C.byref(g)) == impl, kw
+    g = geom(dtype=0, impl=2)
+    assert LIB.sink_swa_select(C.byref(g)) < 0 and b"fp32" in LIB.swa_last_error()
     assert swa.sink_selected_impl(q.float(), q.float(), q.float(), 4, 1) == "simt"
     with pytest.raises(RuntimeError, match="window"):
         swa.sink_selected_impl(q, q, q, 0, 1)
