@@ -20,6 +20,13 @@
 // 255 us.)
 // The maximum a row is scaled by is raised only when it has grown by 2^8, so the accumulator is touched rarely.
 //
+// Measured (bf16, head dims 128, 16 heads on 4): 8192 tokens, window 4096 219 us, 940 TFLOP/s of visible pairs; 16384 tokens, window
+// 1024, 64 sinks 165 us, 850.  Tensor pipe 48 % busy, exponential unit 48 %: a group's chain is what is left (scores to registers 280 cycles,
+// maximum 400, exponentials 1700 beside the other group's, the wait for P V and Q K^T 1400).  Tried and not kept: a part of the exponentials
+// as polynomials on the fp32 pipes (one pair in eight 235 us, in two 287: issue slots, not the exponential unit, run short); reading the
+// scores twice from tensor memory instead of holding 128 in registers (304 us); the running maximum of the block before with a second
+// look (298 us, spills).
+//
 // A hidden pair has P = 0, which is nothing to a sum until the value is an infinity or a NaN: a row that ends as one is done again
 // by row_forward, which touches only what the row sees, after the CTA's last tile.
 //
