@@ -403,6 +403,29 @@ int sink_swa_fwd(const sink_geom_t* g, const swa_tensor_t* q, const swa_tensor_t
   return launch_rows<0>(a, g->dtype, st);
 }
 
+// The softmax delta: rows of whole 16-byte units here, others by the kernels for grids (a sequence is a grid of one column).
+static int launch_delta(const swa::sink::Args& a, const sink_geom_t* g, const swa_tensor_t* o, const swa_tensor_t* d_o, void* stream) {
+  const int e = g->dtype == SWA_F32 ? 4 : 8, units = g->d_v / e;
+  auto whole = [&](const swa_tensor_t* t) {
+    return t->stride[3] == 1 && (uintptr_t)t->ptr % 16 == 0 && t->stride[0] % e == 0 && t->stride[1] % e == 0 && t->stride[2] % e == 0;
+  };
+  if (g->d_v % e || units > 32 || !whole(o) || !whole(d_o)) {
+    if ((int64_t)g->B * g->Hq > 65535) return fail(E_SHAPE, "B*Hq exceeds 65535");
+    swa_geom_t sg;
+    memset(&sg, 0, sizeof(sg));
+    sg.dtype = g->dtype; sg.B = g->B; sg.H = g->Hq; sg.b_size = 1; sg.t_height = g->N; sg.t_width = 1; sg.d_qk = g->d_qk; sg.d_v = g->d_v;
+    sg.sm_scale = g->sm_scale;
+    return swa_bwd_delta(&sg, o, d_o, a.delta, stream);
+  }
+  int group = 1;
+  while (group < units) group *= 2;
+  const int rows = 256 / group * swa::sink::kDeltaRows;
+  const dim3 grid((a.N + rows - 1) / rows, a.Hq, a.B);
+  cudaError_t err = cudaSuccess;
+  SINK_DISPATCH(g->dtype, err = swa::launch_stream(swa::sink::delta_rows_kernel<T>, grid, 256, (cudaStream_t)stream, a, units, group));
+  return launched(err, "sink delta");
+}
+
 static int64_t delta_bytes(const sink_geom_t* g) { return ((int64_t)g->B * g->Hq * g->N * 4 + 255) / 256 * 256; }
 
 static int64_t part_bytes(const sink_geom_t* g, int impl) {
@@ -435,12 +458,7 @@ int sink_swa_bwd(const sink_geom_t* g, const swa_tensor_t* q, const swa_tensor_t
   a.dq = swa::make_view(dq); a.dk = swa::make_view(dk); a.dv = swa::make_view(dv);
   a.lse = const_cast<float*>(lse);
   a.delta = (float*)scratch;
-  swa_geom_t sg;
-  memset(&sg, 0, sizeof(sg));
-  sg.dtype = g->dtype; sg.B = g->B; sg.H = g->Hq; sg.b_size = 1; sg.t_height = g->N; sg.t_width = 1; sg.d_qk = g->d_qk; sg.d_v = g->d_v;
-  sg.sm_scale = g->sm_scale;
-  if ((int64_t)g->B * g->Hq > 65535) return fail(E_SHAPE, "B*Hq exceeds 65535");
-  if (int e = swa_bwd_delta(&sg, o, d_o, a.delta, stream)) return e;
+  if (int e = launch_delta(a, g, o, d_o, stream)) return e;
   if (impl == SWA_IMPL_TC) {
     int launches = 0;
     if (swa::sink::tc_bwd(a, g->dtype, (char*)scratch + delta_bytes(g), status, st, &launches))
