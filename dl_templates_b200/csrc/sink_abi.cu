@@ -129,7 +129,7 @@ bool f32_tiles(const sink_geom_t* g, const swa_tensor_t* const* ts, int n) {
   return true;
 }
 
-// Plan of a kernel: tiles, pieces of the blocks with sinks (KIND 2).  A piece is as long as an ordinary block's stream, G (W + 63) rows.
+// Plan of a kernel: tiles, pieces of the blocks with sinks (KIND 2).
 template <int KIND>
 swa::sink::F32Params f32_plan(const swa::sink::Args& a, float* part) {
   constexpr int R = swa::sink::kF32Rows;
@@ -140,8 +140,10 @@ swa::sink::F32Params f32_plan(const swa::sink::Args& a, float* part) {
   p.part = part;
   if (KIND == 2) {
     p.n_sb = std::min(p.n_t, (a.ns + R - 1) / R);
-    p.piece_len = a.G * ((R - 1 + a.W + R - 1) / R);
-    p.pieces = p.n_sb ? (a.G * p.n_t + p.piece_len - 1) / p.piece_len : 0;
+    const swa::sink::Pieces c = swa::sink::cut_pieces(a, p.n_sb, R, R);
+    p.near = c.near;
+    p.piece_len = c.len;
+    p.pieces = c.most;
     p.n_sink_items = p.n_sb * p.pieces * a.B * a.Hkv;
   }
   return p;
@@ -172,7 +174,7 @@ int launch_f32(const swa::sink::Args& a, float* part, cudaStream_t st) {
   if (int c = launched(e, "sink fp32 tiles")) return c;
   if (KIND != 2 || p.pieces <= 1) return 0;
   constexpr int R = swa::sink::kF32Rows, WARPS = swa::sink::kRowWarps;
-  const swa::sink::JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, R, R, a.dqk + a.dv_dim, 4, part};
+  const swa::sink::JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, p.near, R, R, a.dqk + a.dv_dim, 4, part};
   e = swa::launch_pdl(swa::sink::join_kernel<float>, dim3(std::min(p.n_sb * R, a.N + WARPS - 1) / WARPS, a.Hkv * 8, a.B), 32 * WARPS, 0, st, jp);
   return launched(e, "sink join");
 }

@@ -31,7 +31,7 @@ constexpr int kF32Rows = 64, kF32Threads = 256, kF32PPitch = kF32Rows + 4;
 
 struct F32Params {
   Args a;
-  int n_t, n_sb, pieces, piece_len, n_sink_items;   // KIND 2, as in BwdParams
+  int n_t, n_sb, pieces, piece_len, near, n_sink_items;   // KIND 2: blocks that hold sinks, their pieces (cut_pieces)
   float* part;                                      // [B, Hkv, n_sb, pieces, 64, d_qk + d_v]
 };
 

@@ -243,6 +243,22 @@ __global__ void __launch_bounds__(256) delta_rows_kernel(const __grid_constant__
 // rows into pieces of piece_len, each of which leaves its sums in part [B, Hkv, n_sb, pieces, rows * (d_qk + d_v)], row j and column c of
 // them at j * s_row + c / 4 * s_col4 + c % 4.  Added here in the order of the pieces, one warp per row; a block that is a single piece
 // has gone straight out.
+// Pieces of blocks with sinks: as long as an ordinary block's stream (G * near blocks, near = those that rows other than sinks can see), but
+// no more of them than keep every SM busy four times over, or than keep a piece from outlasting the kernels' waits: what they leave
+// for the join stays below 100 MB or so however long the sequences are.
+struct Pieces { int near, len, most; };
+inline Pieces cut_pieces(const Args& a, int n_sb, int rows, int stream) {
+  Pieces c;
+  c.near = (rows - 1 + a.W + stream - 1) / stream;
+  const int64_t all = (int64_t)a.G * ((a.N + stream - 1) / stream), blocks = (int64_t)a.B * a.Hkv * n_sb;
+  const int64_t busy = (4 * 148 + blocks - 1) / (blocks > 0 ? blocks : 1), patient = ((int64_t)a.G * a.N >> 24) + 1;
+  const int64_t cap = busy > patient ? busy : patient, shortest = (all + cap - 1) / cap, ordinary = (int64_t)a.G * c.near;
+  const int64_t len = ordinary > shortest ? ordinary : shortest;
+  c.len = (int)(len < INT32_MAX ? len : INT32_MAX);
+  c.most = n_sb ? (int)((all + c.len - 1) / c.len) : 0;
+  return c;
+}
+
 // Whether `nb` blocks of the stream from `first` on hold one that rows other than sinks can see: the first `near` of a head's `per_head`.  The
 // other pieces leave sums for the sinks' rows only.
 __device__ __forceinline__ bool piece_near(int first, int nb, int per_head, int near) {
@@ -252,7 +268,7 @@ __device__ __forceinline__ bool piece_near(int first, int nb, int per_head, int 
 
 struct JoinParams {
   Args a;
-  int n_sb, pieces, piece_len, rows, stream, s_row, s_col4;
+  int n_sb, pieces, piece_len, near, rows, stream, s_row, s_col4;
   const float* part;
 };
 
@@ -268,14 +284,14 @@ __global__ void __launch_bounds__(32 * kRowWarps) join_kernel(const __grid_const
   if (j >= a.N || blk >= p.n_sb || x0 >= len || c - lane >= d) return;            // (a block behind the end: zeros, written by its first piece)
   const int all = (len - x0 + p.stream - 1) / p.stream * a.G;
   if (all <= p.piece_len) return;
-  const int pieces = j < len ? (all + p.piece_len - 1) / p.piece_len : 0, per_head = all / a.G, near = p.piece_len / a.G;
+  const int pieces = j < len ? (all + p.piece_len - 1) / p.piece_len : 0, per_head = all / a.G;
   const bool sink = j < a.ns;
   const int64_t step = (int64_t)p.rows * d;
   const float* part = p.part + (((int64_t)b * a.Hkv + hk) * p.n_sb + blk) * p.pieces * step + (j - x0) * p.s_row + (c >> 2) * p.s_col4 + (c & 3);
   float acc = 0.f;
   for (int p0 = 0; p0 < pieces; p0 += 32) {
     const int mine = p0 + lane;
-    uint32_t has = __ballot_sync(0xffffffffu, mine < pieces && (sink || piece_near(mine * p.piece_len, min(p.piece_len, all - mine * p.piece_len), per_head, near)));
+    uint32_t has = __ballot_sync(0xffffffffu, mine < pieces && (sink || piece_near(mine * p.piece_len, min(p.piece_len, all - mine * p.piece_len), per_head, p.near)));
     if (c >= d) has = 0;
     const float* from = part + p0 * step;
 #pragma unroll 1

@@ -126,10 +126,11 @@ int launch_bwd(const Args& a, int dtype, void* scratch, int32_t* status, cudaStr
   if constexpr (KIND == 1) {
     p.n_items = p.n_t * a.B * a.Hq;
   } else {
-    // An ordinary block streams G (W + 127) rows; blocks with sinks, G N rows, are cut into pieces of that length.
     p.n_sb = std::min(p.n_t, (a.ns + kTile - 1) / kTile);
-    p.piece_len = a.G * ((kTile - 1 + a.W + N - 1) / N);
-    p.pieces = p.n_sb ? (a.G * ((a.N + N - 1) / N) + p.piece_len - 1) / p.piece_len : 0;
+    const Pieces c = cut_pieces(a, p.n_sb, kTile, N);
+    p.near = c.near;
+    p.piece_len = c.len;
+    p.pieces = c.most;
     p.n_sink_items = p.n_sb * p.pieces * a.B * a.Hkv;
     p.n_items = p.n_sink_items + (p.n_t - p.n_sb) * a.B * a.Hkv;
     p.part = (float*)scratch;
@@ -151,7 +152,7 @@ int launch_bwd(const Args& a, int dtype, void* scratch, int32_t* status, cudaStr
   if (e == cudaSuccess) e = launch_pdl(kern, dim3(std::min(p.n_items, tc::sm_count())), kThreads, smem, st, txq, txv, tyq, tyv, toq, tov, p);
   if (e == cudaSuccess && KIND == 2 && p.pieces > 1) {
     const dim3 grid(std::min(p.n_sb * kTile, a.N + kRowWarps - 1) / kRowWarps, a.Hkv * 8, a.B);
-    const JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, kTile, N, 4, 4 * kTile, p.part};
+    const JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, p.near, kTile, N, 4, 4 * kTile, p.part};
     e = dtype == SWA_BF16 ? launch_pdl(join_kernel<__nv_bfloat16>, grid, 32 * kRowWarps, 0, st, jp)
                           : launch_pdl(join_kernel<__half>, grid, 32 * kRowWarps, 0, st, jp);
   }

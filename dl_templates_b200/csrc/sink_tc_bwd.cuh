@@ -38,7 +38,7 @@ struct BwdParams {
   Args a;
   int n_items, stages, xbufs;
   int n_t;                                      // tiles of 128 resident rows
-  int n_sb, pieces, piece_len, n_sink_items;    // KIND 2: blocks that hold sinks, pieces of each at most, blocks of a piece
+  int n_sb, pieces, piece_len, near, n_sink_items;    // KIND 2: blocks that hold sinks, their pieces (cut_pieces)
   float* part;                                  // [B, Hkv, n_sb, pieces, 128, d_qk + d_v]
   int32_t* status;
 };
@@ -549,7 +549,7 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
       if (!ok) break;
       tc_fence_after();
       const bool live = w.x0 + r < w.len;
-      const bool counts = KIND == 2 && w.piece >= 0 && (w.x0 + r < a.ns || piece_near(w.first, w.nb, w.per_head, p.piece_len / a.G));
+      const bool counts = KIND == 2 && w.piece >= 0 && (w.x0 + r < a.ns || piece_near(w.first, w.nb, w.per_head, p.near));
       uint64_t z = 0ull;
       // accumulators, 32 columns at a time: dV, then dQ or dK
       constexpr int kV = KIND == 2 ? 2 * VC : 0, kAll = kV + 2 * XC;

@@ -409,9 +409,12 @@ def test_offsets_beyond_32_bits():
 
 def test_largest_sinks_and_one_token_windows():
     """1024 sinks over many blocks, windows of one token, more heads than one MMA tile of the decoding kernel has."""
-    for case in ((1, 2, 1, 1500, 1, 1024, 64, 64, None), (1, 24, 1, 260, 33, 2, 64, 64, [259])):
+    for case, dtype in (((1, 2, 1, 1500, 1, 1024, 64, 64, None), BF), ((1, 24, 1, 260, 33, 2, 64, 64, [259]), BF),
+                        # blocks with sinks in fewer pieces than their length asks for, or in one: so many heads that the SMs are busy
+                        ((2, 40, 40, 1030, 20, 1024, 8, 8, [1030, 1027]), BF), ((1, 150, 150, 700, 1, 4, 8, 8, None), BF),
+                        ((1, 150, 150, 700, 1, 4, 8, 8, None), F32)):
         _, _, _, _, W, ns, _, _, lens = case
-        t, scale = attn_case(case, BF)
+        t, scale = attn_case(case, dtype)
         want, bound = orc.attention(t["q"], t["k"], t["v"], lens, W, ns, scale, t["do"])
         got = run_attn(t, lens_tensor(lens), W, ns, scale)
         for n in want:

@@ -63,6 +63,19 @@ def test_sink_entries_refuse_missing_tensors_and_small_scratch():
         assert b"scratch" in LIB.swa_last_error()
 
 
+@pytest.mark.parametrize("dtype", [0, 2])
+def test_scratch_stays_small(dtype):
+    """Partial sums of the blocks with sinks: below 200 MB beside the softmax delta for any window, sinks and length."""
+    for B, Hq, Hkv in ((1, 1, 1), (1, 16, 4), (8, 64, 8), (64, 32, 32), (3, 8, 1)):
+        for N in (1, 100, 1 << 14, 1 << 17, 1 << 20):
+            for W in (1, 128, 5000):
+                for ns in (0, 1, 4, 130, 1024):
+                    g = geom(dtype=dtype, B=B, Hq=Hq, Hkv=Hkv, N=N, window=W, n_sink=ns, d_qk=128, d_v=128)
+                    extra = LIB.sink_swa_bwd_scratch(C.byref(g)) - 4 * B * Hq * N
+                    assert 0 <= extra < 200 << 20, (B, Hq, Hkv, N, W, ns, extra)
+                    assert ns or extra < 256
+
+
 def test_rope_axes_are_refused():
     t = tensor4()
     ok = dict(pos=1 << 20, stride=(0, 100), n_axes=2, pairs=(8, 8, 0, 0), rows=(10, 10, 0, 0), cs=(1 << 20, 1 << 20, 0, 0))
