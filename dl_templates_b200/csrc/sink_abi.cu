@@ -132,7 +132,7 @@ bool f32_tiles(const sink_geom_t* g, const swa_tensor_t* const* ts, int n) {
 // Plan of a kernel: tiles, pieces of the blocks with sinks (KIND 2).
 template <int KIND>
 swa::sink::F32Params f32_plan(const swa::sink::Args& a, float* part) {
-  constexpr int R = swa::sink::kF32Rows;
+  constexpr int R = swa::sink::kF32X;
   swa::sink::F32Params p;
   memset(&p, 0, sizeof(p));
   p.a = a;
@@ -140,7 +140,7 @@ swa::sink::F32Params f32_plan(const swa::sink::Args& a, float* part) {
   p.part = part;
   if (KIND == 2) {
     p.n_sb = std::min(p.n_t, (a.ns + R - 1) / R);
-    const swa::sink::Pieces c = swa::sink::cut_pieces(a, p.n_sb, R, R);
+    const swa::sink::Pieces c = swa::sink::cut_pieces(a, p.n_sb, R, swa::sink::kF32Rows);
     p.near = c.near;
     p.piece_len = c.len;
     p.pieces = c.most;
@@ -150,7 +150,7 @@ swa::sink::F32Params f32_plan(const swa::sink::Args& a, float* part) {
 }
 int64_t f32_scratch(const swa::sink::Args& a) {
   const swa::sink::F32Params p = f32_plan<2>(a, nullptr);
-  return p.pieces > 1 ? (int64_t)a.B * a.Hkv * p.n_sb * p.pieces * swa::sink::kF32Rows * (a.dqk + a.dv_dim) * 4 : 0;
+  return p.pieces > 1 ? (int64_t)a.B * a.Hkv * p.n_sb * p.pieces * swa::sink::kF32X * (a.dqk + a.dv_dim) * 4 : 0;
 }
 
 template <int KIND, int DQ, int DV>
@@ -173,8 +173,8 @@ int launch_f32(const swa::sink::Args& a, float* part, cudaStream_t st) {
                               : a.dv_dim <= 64 ? launch_f32_as<KIND, 128, 64>(p, items, st) : launch_f32_as<KIND, 128, 128>(p, items, st);
   if (int c = launched(e, "sink fp32 tiles")) return c;
   if (KIND != 2 || p.pieces <= 1) return 0;
-  constexpr int R = swa::sink::kF32Rows, WARPS = swa::sink::kRowWarps;
-  const swa::sink::JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, p.near, R, R, a.dqk + a.dv_dim, 4, part};
+  constexpr int R = swa::sink::kF32X, WARPS = swa::sink::kRowWarps;
+  const swa::sink::JoinParams jp{a, p.n_sb, p.pieces, p.piece_len, p.near, R, swa::sink::kF32Rows, a.dqk + a.dv_dim, 4, part};
   e = swa::launch_pdl(swa::sink::join_kernel<float>, dim3(std::min(p.n_sb * R, a.N + WARPS - 1) / WARPS, a.Hkv * 8, a.B), 32 * WARPS, 0, st, jp);
   return launched(e, "sink join");
 }

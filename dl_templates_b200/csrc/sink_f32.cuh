@@ -1,17 +1,18 @@
 // fp32 kernels of the attention with a sliding window and sink tokens, on the CUDA cores: KIND 0 forward, 1 dQ, 2 dK / dV (the products
 // are those of sink_tc_fwd.cuh and sink_tc_bwd.cuh).
 //
-// A block of 256 threads holds 64 resident rows and streams blocks of 64 rows of the other side through shared memory.  Thread
-// (ty, tx) owns the scores of rows ty + 16 i and columns tx + 16 j, i, j < 4, and columns 4 tx + 64 c of the accumulators of the
+// A block of 128 threads holds 32 resident rows and streams blocks of 64 rows of the other side through shared memory.  Thread
+// (ty, tx) owns the scores of rows ty + 8 i and columns tx + 16 j, i, j < 4, and columns 4 tx + 64 c of the accumulators of the
 // same rows: a row belongs to one half warp, so that maxima and sums are shuffles and the weights go from the scores'
 // threads to the second product's through shared memory without a barrier.  Rows in shared memory are 4 floats longer than the
 // head: 16 rows read at the same column then lie in different banks.
 // Bound by the fp32 pipes: 8 16-byte loads feed 64 multiply-adds, issued as 32 packed ones.
 //
-// Measured: 4000 tokens, window 1000, 16 heads of 128: forward 1.94 ms (30 TFLOP/s of 74 nominal), backward 6.5 ms; the fp32 pipes 50 to 54 % busy.  Tried
-// and not kept: 512 threads a block with half the rows each (777 tokens, 8 heads of 64: 46 us instead of 40), scalar multiply-adds in the
-// second product (2.02 ms).  Tensor cores (three tf32 products for one) would accumulate with truncation, over a whole window to
-// 1e-5 and more: not what a caller of fp32 asks for.
+// Measured: 4000 tokens, window 1000, 16 heads of 128, batch 2: forward 1.88 ms (31 TFLOP/s of 74 nominal), backward 6.2 ms; 777 tokens, window 256, 8
+// heads of 64 33 and 103 us.  With 64 resident rows and 256 threads 1.93 and 6.5 ms, 40 and 115 us: fewer and longer blocks (the fp32 pipes 50 to
+// 54 % busy; 753 tokens, d_v = 128, 128 heads the other way round, 413 us against 446).  Tried and not kept beside that: 512 threads for 64 rows
+// (46 us), scalar multiply-adds in the second product (2.02 ms).  Tensor cores (three tf32 products for one) would accumulate with
+// truncation, over a whole window to 1e-5 and more: not what a caller of fp32 asks for.
 //
 // Neither started early under their predecessor nor letting their successor start: blocks of a small grid that start while the one before
 // is still running are packed two and three to an SM onto the SMs that it left idle, and stay there (104 blocks each: 230 us a
@@ -27,7 +28,8 @@
 namespace swa {
 namespace sink {
 
-constexpr int kF32Rows = 64, kF32Threads = 256, kF32PPitch = kF32Rows + 4;
+constexpr int kF32X = 32, kF32Rows = 64, kF32Threads = 4 * kF32X, kF32PPitch = kF32Rows + 4;      // resident, streamed rows
+constexpr int kF32Y = kF32Threads / 16;           // rows ty + kF32Y i of a thread
 
 struct F32Params {
   Args a;
@@ -38,15 +40,16 @@ struct F32Params {
 template <int KIND, int DQ, int DV>
 struct F32Shape {
   static constexpr int PQ = DQ + 4, PV = DV + 4;
-  static constexpr int kX = kF32Rows * (PQ + (KIND ? PV : 0)), kY = kF32Rows * (PQ + PV);
-  static constexpr int kSmem = 4 * (kX + kY + kF32Rows * kF32PPitch);
+  static constexpr int kX = kF32X * (PQ + (KIND ? PV : 0)), kY = kF32Rows * (PQ + PV);
+  static constexpr int kSmem = 4 * (kX + kY + kF32X * kF32PPitch);
 };
 
 // 64 rows of a [B, H, N, d] tensor from row `n0` on into rows of `pitch` floats; zeros behind the last row and the last element.
+template <int ROWS>
 __device__ __forceinline__ void f32_load(float* s, int pitch, int dmax, const View4& t, int b, int h, int n0, int N, int d) {
   const float* p = (const float*)t.ptr + b * t.s0 + h * t.s1;
   const int units = dmax / 4;
-  for (int x = threadIdx.x; x < kF32Rows * units; x += kF32Threads) {
+  for (int x = threadIdx.x; x < ROWS * units; x += kF32Threads) {
     const int r = x / units, c = x % units * 4;
     const bool on = n0 + r < N && c < d;
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(s + r * pitch + c)),
@@ -54,7 +57,7 @@ __device__ __forceinline__ void f32_load(float* s, int pitch, int dmax, const Vi
   }
 }
 
-// acc[i][j] = x row (ty + 16 i) . y row (tx + 16 j)
+// acc[i][j] = x row (ty + kF32Y i) . y row (tx + 16 j)
 template <int D>
 __device__ __forceinline__ void f32_scores(float (*acc)[4], const float* x, const float* y, int ty, int tx) {
   using namespace ptx;
@@ -67,7 +70,7 @@ __device__ __forceinline__ void f32_scores(float (*acc)[4], const float* x, cons
   for (int c = 0; c < D; c += 4) {
     ulonglong2 p[4], q[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const ulonglong2*>(x + (ty + 16 * i) * (D + 4) + c);
+    for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const ulonglong2*>(x + (ty + kF32Y * i) * (D + 4) + c);
 #pragma unroll
     for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const ulonglong2*>(y + (tx + 16 * j) * (D + 4) + c);
 #pragma unroll
@@ -84,7 +87,7 @@ __device__ __forceinline__ void f32_scores(float (*acc)[4], const float* x, cons
     }
 }
 
-// acc[i][2 c + e] (pairs of columns 4 tx + 64 c + 2 e) += w row (ty + 16 i) . y columns
+// acc[i][2 c + e] (pairs of columns 4 tx + 64 c + 2 e) += w row (ty + kF32Y i) . y columns
 template <int D>
 __device__ __forceinline__ void f32_product(uint64_t (*acc)[D / 32], const float* w, const float* y, int ty, int tx) {
   using namespace ptx;
@@ -92,7 +95,7 @@ __device__ __forceinline__ void f32_product(uint64_t (*acc)[D / 32], const float
   for (int k = 0; k < kF32Rows; k += 4) {
     float p[4][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(p[i]) = *reinterpret_cast<const float4*>(w + (ty + 16 * i) * kF32PPitch + k);
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(p[i]) = *reinterpret_cast<const float4*>(w + (ty + kF32Y * i) * kF32PPitch + k);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -109,12 +112,12 @@ __device__ __forceinline__ void f32_product(uint64_t (*acc)[D / 32], const float
 }
 
 template <int KIND, int DQ, int DV>
-__global__ void __launch_bounds__(kF32Threads, KIND == 2 && DQ + DV > 128 ? 1 : 2) f32_kernel(const __grid_constant__ F32Params p) {
+__global__ void __launch_bounds__(kF32Threads, (KIND == 2 && DQ + DV > 128 ? 1 : 2) * 256 / kF32Threads) f32_kernel(const __grid_constant__ F32Params p) {
   using namespace ptx;
   using S = F32Shape<KIND, DQ, DV>;
   extern __shared__ __align__(16) float f32_smem[];
-  __shared__ int bad_row[kF32Rows];
-  float *xq = f32_smem, *xv = xq + kF32Rows * S::PQ, *yq = f32_smem + S::kX, *yv = yq + kF32Rows * S::PQ, *ws = yv + kF32Rows * S::PV;
+  __shared__ int bad_row[kF32X];
+  float *xq = f32_smem, *xv = xq + kF32X * S::PQ, *yq = f32_smem + S::kX, *yv = yq + kF32Rows * S::PQ, *ws = yv + kF32Rows * S::PV;
   const Args& a = p.a;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
 
@@ -124,7 +127,7 @@ __global__ void __launch_bounds__(kF32Threads, KIND == 2 && DQ + DV > 128 ? 1 : 
     const int per = a.B * a.Hq, r = blockIdx.x % per;
     b = r / a.Hq;
     h = r % a.Hq;
-    x0 = (p.n_t - 1 - (int)(blockIdx.x / per)) * kF32Rows;
+    x0 = (p.n_t - 1 - (int)(blockIdx.x / per)) * kF32X;
   } else {
     const int per = a.B * a.Hkv;
     int r, blk, pc = 0;
@@ -138,18 +141,18 @@ __global__ void __launch_bounds__(kF32Threads, KIND == 2 && DQ + DV > 128 ? 1 : 
     }
     b = r / a.Hkv;
     h = r % a.Hkv;
-    x0 = blk * kF32Rows;
+    x0 = blk * kF32X;
     piece = pc;
   }
   const int len = seq_len(a, b);
   if constexpr (KIND != 2) {
-    hi = x0 / kF32Rows;
+    hi = min(x0 + kF32X - 1, max(len, 1) - 1) / kF32Rows;
     lo = max(0, x0 - a.W + 1) / kF32Rows;
     sb = min((a.ns + kF32Rows - 1) / kF32Rows, lo);
     nb = x0 < len ? hi - lo + 1 + sb : 0;
   } else {
-    const bool sink_block = x0 / kF32Rows < p.n_sb;
-    const int end = sink_block ? len : (int)min((int64_t)len, (int64_t)x0 + kF32Rows - 1 + a.W);
+    const bool sink_block = x0 / kF32X < p.n_sb;
+    const int end = sink_block ? len : (int)min((int64_t)len, (int64_t)x0 + kF32X - 1 + a.W);
     per_head = x0 < len ? (end - x0 + kF32Rows - 1) / kF32Rows : 0;
     const int all = per_head * a.G;
     if (sink_block) {
@@ -166,14 +169,14 @@ __global__ void __launch_bounds__(kF32Threads, KIND == 2 && DQ + DV > 128 ? 1 : 
   const View4 &tq = KIND == 2 ? a.k : a.q, &tv = KIND == 2 ? a.v : a.d_o;          // resident
   const View4 &sq = KIND == 2 ? a.q : a.k, &sv = KIND == 2 ? a.d_o : a.v;          // streamed
   if (nb) {
-    f32_load(xq, S::PQ, DQ, tq, b, h, x0, a.N, a.dqk);
-    if constexpr (KIND != 0) f32_load(xv, S::PV, DV, tv, b, h, x0, a.N, a.dv_dim);
+    f32_load<kF32X>(xq, S::PQ, DQ, tq, b, h, x0, a.N, a.dqk);
+    if constexpr (KIND != 0) f32_load<kF32X>(xv, S::PV, DV, tv, b, h, x0, a.N, a.dv_dim);
   }
   // statistics of the resident rows (KIND 0 running, 1 given)
   float m[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int x = x0 + ty + 16 * i;
+    const int x = x0 + ty + kF32Y * i;
     m[i] = KIND == 0 ? -INFINITY : 0.f;
     l[i] = 0.f;
     if (KIND == 1 && x < len) {
@@ -201,8 +204,8 @@ __global__ void __launch_bounds__(kF32Threads, KIND == 2 && DQ + DV > 128 ? 1 : 
       hy = h * a.G + (first + n) / per_head;
     }
     __syncthreads();                                             // the block before has been read
-    f32_load(yq, S::PQ, DQ, sq, b, hy, y0, a.N, a.dqk);
-    f32_load(yv, S::PV, DV, sv, b, hy, y0, a.N, a.dv_dim);
+    f32_load<kF32Rows>(yq, S::PQ, DQ, sq, b, hy, y0, a.N, a.dqk);
+    f32_load<kF32Rows>(yv, S::PV, DV, sv, b, hy, y0, a.N, a.dv_dim);
     asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     float s[4][4];
@@ -212,7 +215,7 @@ __global__ void __launch_bounds__(kF32Threads, KIND == 2 && DQ + DV > 128 ? 1 : 
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int x = x0 + ty + 16 * i, y = y0 + tx + 16 * j, qi = KIND == 2 ? y : x, kj = KIND == 2 ? x : y;
+        const int x = x0 + ty + kF32Y * i, y = y0 + tx + 16 * j, qi = KIND == 2 ? y : x, kj = KIND == 2 ? x : y;
         if (kj <= qi && qi < len && (kj > qi - a.W || kj < a.ns)) see |= 1u << (4 * i + j);
       }
     if constexpr (KIND == 0) {
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(kF32Threads, KIND == 2 && DQ + DV > 128 ? 1 : 
         for (int j = 0; j < 4; ++j) {
           const float w = s[i][j] == -INFINITY ? 0.f : exp2f(s[i][j] - mn);
           sum += w;
-          ws[(ty + 16 * i) * kF32PPitch + tx + 16 * j] = w;
+          ws[(ty + kF32Y * i) * kF32PPitch + tx + 16 * j] = w;
         }
 #pragma unroll
         for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -264,7 +267,7 @@ __global__ void __launch_bounds__(kF32Threads, KIND == 2 && DQ + DV > 128 ? 1 : 
           const bool on = see >> (4 * i + j) & 1u;
           const float w = on ? exp2f(fmaf(s[i][j], a.c2, -(KIND == 1 ? m[i] : ly[j]))) : 0.f;
           dp[i][j] = on ? w * (dp[i][j] - (KIND == 1 ? l[i] : dy[j])) : 0.f;
-          ws[(ty + 16 * i) * kF32PPitch + tx + 16 * j] = KIND == 1 ? dp[i][j] : w;
+          ws[(ty + kF32Y * i) * kF32PPitch + tx + 16 * j] = KIND == 1 ? dp[i][j] : w;
         }
       __syncwarp();
       if constexpr (KIND == 2) {
@@ -273,7 +276,7 @@ __global__ void __launch_bounds__(kF32Threads, KIND == 2 && DQ + DV > 128 ? 1 : 
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) ws[(ty + 16 * i) * kF32PPitch + tx + 16 * j] = dp[i][j];
+          for (int j = 0; j < 4; ++j) ws[(ty + kF32Y * i) * kF32PPitch + tx + 16 * j] = dp[i][j];
         __syncwarp();
       }
       f32_product<DQ>(acq, ws, yq, ty, tx);
@@ -283,10 +286,10 @@ __global__ void __launch_bounds__(kF32Threads, KIND == 2 && DQ + DV > 128 ? 1 : 
 
   // ---- store
   __syncthreads();
-  if (threadIdx.x < kF32Rows) bad_row[threadIdx.x] = 0;
+  if (threadIdx.x < kF32X) bad_row[threadIdx.x] = 0;
   __syncthreads();
   auto put = [&](auto& v, const View4& t, int dmax, int d, float* part, int i, float f) {
-    const int r = ty + 16 * i, x = x0 + r;
+    const int r = ty + kF32Y * i, x = x0 + r;
     float z = 0.f;
     for (int c = 0; c < dmax / 64; ++c) {
       const int col = 4 * tx + 64 * c;
@@ -300,10 +303,10 @@ __global__ void __launch_bounds__(kF32Threads, KIND == 2 && DQ + DV > 128 ? 1 : 
     }
     if (!part && x < len && !(z == 0.f)) bad_row[r] = 1;
   };
-  float* part = KIND == 2 && piece >= 0 ? p.part + (((((int64_t)b * a.Hkv + h) * p.n_sb + x0 / kF32Rows) * p.pieces + piece) * kF32Rows) * (a.dqk + a.dv_dim) : nullptr;
+  float* part = KIND == 2 && piece >= 0 ? p.part + (((((int64_t)b * a.Hkv + h) * p.n_sb + x0 / kF32X) * p.pieces + piece) * kF32X) * (a.dqk + a.dv_dim) : nullptr;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int x = x0 + ty + 16 * i;
+    const int x = x0 + ty + kF32Y * i;
     if constexpr (KIND == 0) {
       put(acc, a.o, DV, a.dv_dim, nullptr, i, x < len ? 1.f / l[i] : 0.f);
       if (tx == 0 && x < a.N) a.lse[((int64_t)b * a.Hq + h) * a.N + x] = x < len ? m[i] + log2f(l[i]) : -INFINITY;
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(kF32Threads, KIND == 2 && DQ + DV > 128 ? 1 : 
   __syncthreads();
   float* s = f32_smem + (threadIdx.x >> 5) * 2 * kMaxDim;        // (the tiles are done with)
 #pragma unroll 1
-  for (int r = threadIdx.x >> 5; r < kF32Rows; r += kF32Threads / 32) {
+  for (int r = threadIdx.x >> 5; r < kF32X; r += kF32Threads / 32) {
     if (!bad_row[r]) continue;
     if constexpr (KIND == 0) row_forward<float>(a, b, h, x0 + r, s);
     if constexpr (KIND == 1) row_dq<float>(a, b, h, x0 + r, s);
