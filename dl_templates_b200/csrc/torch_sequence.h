@@ -26,19 +26,59 @@ void check_writable(const Tensor& t, const char* name) {
     TORCH_CHECK_VALUE(t.size(i) == 1 || t.stride(i) > 0, name, " is an expanded tensor: its elements share memory");
 }
 
+// Sizes reach the kernels as 32-bit numbers.
+void check_sizes(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    for (const int64_t n : t->sizes()) TORCH_CHECK_VALUE(n <= INT32_MAX, "a tensor of shape ", t->sizes(), " is too large");
+}
+
+// An output the caller gives: blocks write it while others still read the inputs, so that it shares no memory with them.  (Views
+// that interleave in one buffer pass: strides alone do not tell.)
+void check_apart(const Tensor& out, std::initializer_list<const Tensor*> others, const char* name) {
+  for (const Tensor* t : others) {
+    if (!t->defined() || !t->numel() || !out.numel()) continue;
+    const at::MemOverlapStatus s = at::get_overlap_status(out, *t);
+    TORCH_CHECK_VALUE(s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial && out.data_ptr() != t->data_ptr(), name,
+                      " shares memory with another tensor of the call");
+  }
+}
+
+// Tells autograd that a tensor it may have saved was written.
+void written(const Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+bool capturing(const c10::Stream& s) {
+  const cudaStream_t stream = c10::cuda::CUDAStream(s).stream();
+  if (!stream) return false;                                     // the default stream never is
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  C10_CUDA_CHECK(cudaStreamIsCapturing(stream, &st));
+  return st != cudaStreamCaptureStatusNone;
+}
+
 // While a graph is captured, autograd's engine would record events on the stream that an older graph's leaf accumulators live on,
-// which is not part of the capture; what follows ends the process inside the engine.  Refused here, while nothing has been launched.
+// which is not part of the capture; what follows ends the process inside the engine.  Refused here, while nothing has been launched:
+// for every leaf that the inputs come from, since all of them take part in the backward pass.
 void check_capture(std::initializer_list<const Tensor*> inputs) {
   for (const Tensor* t : inputs)
     if (!t->is_cuda()) return;                                   // (refused further on)
   const c10::cuda::OptionalCUDAGuard guard((*inputs.begin())->device());
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  std::vector<std::shared_ptr<torch::autograd::Node>> todo;
   for (const Tensor* t : inputs) {
-    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-    const auto acc = torch::autograd::impl::try_get_grad_accumulator(*t);
-    if (!acc) continue;
-    const auto s = acc->stream();
-    TORCH_CHECK(!s.has_value() || *s == c10::cuda::getCurrentCUDAStream(t->get_device()).unwrap(),
+    if (!t->defined() || !t->requires_grad()) continue;
+    if (auto n = t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t)) todo.push_back(std::move(n));
+  }
+  std::unordered_set<const torch::autograd::Node*> seen;
+  while (!todo.empty()) {
+    const std::shared_ptr<torch::autograd::Node> n = std::move(todo.back());
+    todo.pop_back();
+    if (!seen.insert(n.get()).second) continue;
+    for (const torch::autograd::Edge& e : n->next_edges())
+      if (e.function) todo.push_back(e.function);
+    if (!dynamic_cast<const torch::autograd::AccumulateGrad*>(n.get())) continue;
+    const std::optional<c10::Stream> s = n->stream();
+    TORCH_CHECK(!s.has_value() || capturing(*s),
                 "a leaf of this call belongs to an autograd graph recorded on another stream that is still alive; its backward pass "
                 "cannot be captured: drop that graph (its outputs and losses) before capturing, or capture with detached leaves");
   }
@@ -95,10 +135,12 @@ std::array<Tensor, 2> rotate_axes(const Tensor& x, const Tensor& x2, Axes ax, bo
   poll_status();
   check_cuda({&x, &x2}, "q and k");
   TORCH_CHECK_VALUE(x.dim() == 4, "expected [B,H,N,C]");
+  check_sizes({&x});
   const int32_t dt = dtype_code(x.scalar_type());
   if (x2.defined()) {
     TORCH_CHECK_VALUE(x2.dim() == 4 && x2.size(0) == x.size(0) && x2.size(2) == x.size(2) && x2.size(3) == x.size(3),
                       "q and k must agree in batch, tokens and head dim: ", x.sizes(), " beside ", x2.sizes());
+    check_sizes({&x2});
     TORCH_CHECK_TYPE(x2.scalar_type() == x.scalar_type(), "q and k must share a dtype");
   }
   TORCH_CHECK_VALUE(ax.pos.defined(), "positions expected");
@@ -167,7 +209,6 @@ struct SinkWin {
 };
 
 sink_geom_t sink_geom(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lens, const SinkWin& w, int32_t impl) {
-  TORCH_CHECK_VALUE(q.size(2) <= INT32_MAX, "too many tokens");
   return sink_geom_t{dtype_code(q.scalar_type()), (int32_t)q.size(0), (int32_t)q.size(1), (int32_t)k.size(1), (int32_t)q.size(2),
                      (int32_t)q.size(3), (int32_t)v.size(3), w.window, w.n_sink, w.sm, forced_impl(impl),
                      lens.defined() ? lens.data_ptr<int32_t>() : nullptr};
@@ -180,6 +221,7 @@ void check_sink(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
                         k.size(3) == q.size(3) && v.size(0) == k.size(0) && v.size(1) == k.size(1) && v.size(2) == k.size(2),
                     "expected q [B,Hq,N,d_qk], k [B,Hkv,N,d_qk] and v [B,Hkv,N,d_v]");
   TORCH_CHECK_VALUE(k.size(1) > 0 && q.size(1) % k.size(1) == 0, "the heads of q must be a multiple of the heads of k and v");
+  check_sizes({&q, &k, &v});
   TORCH_CHECK_TYPE(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(), "q, k, v must share a dtype");
 }
 
@@ -196,6 +238,7 @@ Fwd sink_forward(Tensor q, Tensor k, Tensor v, Tensor lens, const SinkWin& w, in
   if (out.defined()) {
     check_out(out, shape, q, "out");
     check_writable(out, "out");
+    check_apart(out, {&q, &k, &v}, "out");
   }
   const int64_t pq = sink_padded(q, impl), pv = sink_padded(v, impl);
   if (pq != q.size(3) || pv != v.size(3)) {
@@ -211,6 +254,7 @@ Fwd sink_forward(Tensor q, Tensor k, Tensor v, Tensor lens, const SinkWin& w, in
   f.lse = new_lse(q);
   const sink_geom_t g = sink_geom(q, k, v, lens, w, impl);
   const swa_tensor_t tq = view4(q), tk = view4(k), tv = view4(v), to = view4(f.o);
+  if (out.defined()) written(out);
   check(sink_swa_fwd(&g, &tq, &tk, &tv, &to, f.lse.data_ptr<float>(), status_ptr(q.get_device()), stream_of(q)), "sink_swa_fwd");
   debug_sync();
   return f;
@@ -236,6 +280,9 @@ Grads sink_backward(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor d
     check_out(out.dk, k.sizes(), k, "dk");
     check_out(out.dv, v.sizes(), v, "dv");
     check_writable(out.dq, "dq"); check_writable(out.dk, "dk"); check_writable(out.dv, "dv");
+    check_apart(out.dq, {&q, &k, &v, &o, &d_o, &lse, &out.dk, &out.dv}, "dq");
+    check_apart(out.dk, {&q, &k, &v, &o, &d_o, &lse, &out.dv}, "dk");
+    check_apart(out.dv, {&q, &k, &v, &o, &d_o, &lse}, "dv");
   }
   const int64_t pq = sink_padded(q, impl), pv = sink_padded(v, impl);
   if (pq != q.size(3) || pv != v.size(3)) {
@@ -257,6 +304,8 @@ Grads sink_backward(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor d
   const Tensor scratch = at::empty({bytes}, q.options().dtype(at::kByte));
   const swa_tensor_t tq = view4(q), tk = view4(k), tv = view4(v), to = view4(o), tdo = view4(d_o), tdq = view4(r.dq), tdk = view4(r.dk),
                      tdv = view4(r.dv);
+  if (given)
+    for (const Tensor* t : {&out.dq, &out.dk, &out.dv}) written(*t);
   check(sink_swa_bwd(&g, &tq, &tk, &tv, &to, &tdo, lse.data_ptr<float>(), &tdq, &tdk, &tdv, scratch.data_ptr(), bytes,
                      status_ptr(q.get_device()), stream_of(q)), "sink_swa_bwd");
   debug_sync();
@@ -341,11 +390,15 @@ Tensor kv_append(const Tensor& q, const Tensor& k, const Tensor& v, Axes ax, con
     TORCH_CHECK_VALUE(q.dim() == 4 && q.size(0) == B && q.size(2) == T && q.size(3) == k.size(3), "expected q [B,Hq,T,d_qk]");
     TORCH_CHECK_TYPE(q.scalar_type() == k.scalar_type(), "q, k, v must share a dtype");
   }
+  check_sizes({&k, &v});
+  if (q.defined()) check_sizes({&q});
   const int32_t dt = dtype_code(k.scalar_type());
   check_cuda({&k, &q, &v, &fresh}, "q, k, v and new_lens");
   sink_cache_t c = cache_view(kc, vc, table, lens, B, k.size(1), k.size(3), v.size(3), k);
   check_writable(kc, "k_cache");
   check_writable(vc, "v_cache");
+  check_apart(kc, {&q, &k, &v, &vc}, "k_cache");
+  check_apart(vc, {&q, &k, &v}, "v_cache");
   fresh = int_vector(fresh, B, "new_lens");
   const rope_axes_t r = axes_view(ax, B, T, k);
   const c10::cuda::OptionalCUDAGuard guard(k.device());
@@ -357,12 +410,11 @@ Tensor kv_append(const Tensor& q, const Tensor& k, const Tensor& v, Axes ax, con
     tqo = view4(q_out);
   }
   const swa_tensor_t tk = view4(k), tv = view4(v);
-  TORCH_CHECK_VALUE(T <= INT32_MAX && B <= INT32_MAX, "too many tokens");
   check(kv_append_rope(dt, &r, (int32_t)B, q.defined() ? (int32_t)q.size(1) : 0, (int32_t)k.size(1), (int32_t)T, (int32_t)k.size(3),
                        (int32_t)v.size(3), q.defined() ? &tq : nullptr, q.defined() ? &tqo : nullptr, &tk, &tv, &c,
                        fresh.defined() ? fresh.data_ptr<int32_t>() : nullptr, stream_of(k)), "kv_append_rope");
-  for (const Tensor* t : {&kc, &vc})
-    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  written(kc);
+  written(vc);
   return q_out;
 }
 
@@ -372,6 +424,7 @@ Tensor sink_decode(const Tensor& q, const Tensor& kc, const Tensor& vc, Tensor t
   TORCH_CHECK_VALUE(q.dim() == 4 && q.size(2) == 1, "expected q [B,Hq,1,d_qk], one new token of each sequence");
   TORCH_CHECK_VALUE(kc.dim() == 4 && vc.dim() == 4 && kc.size(1) > 0 && q.size(1) % kc.size(1) == 0,
                     "the heads of q must be a multiple of the heads of the cache");
+  check_sizes({&q, &kc, &vc});
   const int32_t dt = dtype_code(q.scalar_type());
   const sink_cache_t c = cache_view(kc, vc, table, lens, q.size(0), kc.size(1), q.size(3), vc.size(3), q);
   const std::array<int64_t, 4> shape{q.size(0), q.size(1), 1, vc.size(3)};
@@ -379,6 +432,8 @@ Tensor sink_decode(const Tensor& q, const Tensor& kc, const Tensor& vc, Tensor t
   if (out.defined()) {
     check_out(out, shape, q, "out");
     check_writable(out, "out");
+    check_apart(out, {&q, &kc, &vc}, "out");
+    written(out);
   } else {
     out = at::empty(shape, q.options());
   }

@@ -34,5 +34,5 @@ def kv_append_rope(q, k, v, positions, tables, k_cache, v_cache, page_table, seq
 def sink_swa_decode(q, k_cache, v_cache, page_table, seq_lens, window, n_sink, sm_scale=1.0, impl="auto", out=None):
     """Attention of one new token per sequence: ``q [B,Hq,1,d_qk]`` stands at position ``seq_lens[b] - 1`` (its key and value are in the cache
     already) and sees positions ``p >= seq_lens[b] - window`` and ``p < n_sink``.  Returns ``o [B,Hq,1,d_v]`` (``out``: a tensor to write it
-    into); zeros for a sequence of no tokens."""
+    into, apart from ``q`` and the cache); zeros for a sequence of no tokens."""
     return _native.sink_decode(q, k_cache, v_cache, page_table, seq_lens, window, n_sink, sm_scale, _lib.impl_code(impl), out)

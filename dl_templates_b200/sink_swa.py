@@ -23,17 +23,18 @@ import torch
 from . import _lib
 from ._lib import native as _native
 
-MAX_SINKS = 1024                    # SINK_MAX_SINKS of include/swa2d.h
+MAX_SINKS = 1024                    # SINK_MAX_SINKS of include/swa_sequence.h
 
 
 def sink_swa_forward(q, k, v, window, n_sink, sm_scale, seq_lens=None, impl="auto", out=None):
     """Returns ``(o, lse)``, ``lse`` fp32 ``[B,Hq,N]`` in the base-2 domain (``-inf`` for rows behind a sequence's end).  ``out``: an
-    optional ``[B,Hq,N,d_v]`` tensor or strided view that O is written into."""
+    optional ``[B,Hq,N,d_v]`` tensor or strided view that O is written into; it shares no memory with the inputs."""
     return _native.sink_forward(q, k, v, seq_lens, window, n_sink, sm_scale, _lib.impl_code(impl), out)
 
 
 def sink_swa_backward(q, k, v, o, lse, do, window, n_sink, sm_scale, seq_lens=None, impl="auto", out=None):
-    """Returns ``(dq, dk, dv)`` in the input dtype; ``out``: optional ``(dq, dk, dv)`` tensors or strided views to write into."""
+    """Returns ``(dq, dk, dv)`` in the input dtype; ``out``: optional ``(dq, dk, dv)`` tensors or strided views to write
+    into, which share no memory with one another or with the inputs."""
     return _native.sink_backward(q, k, v, o, lse, do, seq_lens, window, n_sink, sm_scale, _lib.impl_code(impl), *(out or (None,) * 3))
 
 

@@ -2,6 +2,7 @@
  * swa_sequence.h -- C ABI of the operators for token sequences: rotary positions with several axes, attention with a sliding
  * window and sink tokens, and the paged cache that serves both.  Same library and conventions as swa2d.h: device pointers and
  * element strides, work enqueued on `stream`, 0 = enqueued, negative = refused before any launch (swa_last_error()).
+ * What a call writes shares no memory with what it reads.
  *
  * Head dims: the CUDA-core kernels take up to 256, the tensor-core kernels multiples of 8 up to 128 in fp16 / bf16.
  */

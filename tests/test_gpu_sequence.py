@@ -508,6 +508,74 @@ def test_training_step_in_a_graph_and_two_graphs():
     assert torch.equal(step(x, do)[0], eager[0][0])
 
 
+def test_capture_beside_a_live_graph_of_an_upstream_leaf():
+    """The leaf whose eager graph lives lies behind other operations: refused all the same; without that graph the capture works, on two
+    streams of one capture too."""
+    g = gen(14)
+    w = randn(g, 1, 2, 200, 64).to(DEV).requires_grad_()
+    k, v = (randn(g, 1, 2, 200, 64).to(DEV) for _ in range(2))
+    rope = swa.RotaryPositionEncodingAxes((32,), (200,)).to(DEV)
+    pos = torch.arange(200, dtype=torch.int32, device=DEV)[None]
+
+    def loss():
+        qr, kr = rope(w * 2, k, pos)
+        return swa.SinkSwa.apply(qr, kr, v, None, 50, 4, 0.125)
+    want, = torch.autograd.grad(loss(), w, torch.ones_like(k))
+    alive = w * 2
+    graph, stream, fork = torch.cuda.CUDAGraph(), torch.cuda.Stream(), torch.cuda.Stream()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(graph, stream=stream):
+            loss()
+    del alive
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        scaled = w * 2                                           # w's accumulator belongs to the captured stream from here on
+        fork.wait_stream(stream)
+        with torch.cuda.stream(fork):
+            qr, kr = rope(scaled, k, pos)
+            o = swa.SinkSwa.apply(qr, kr, v, None, 50, 4, 0.125)
+        stream.wait_stream(fork)
+        got, = torch.autograd.grad(o, w, torch.ones_like(k))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_outputs_share_no_memory_and_count_as_written():
+    g = gen(15)
+    q, k, v = (randn(g, 1, 2, 40, 64).to(DEV) for _ in range(3))
+    o, lse = swa.sink_swa_forward(q, k, v, 9, 2, 0.125)
+    both = torch.empty(2, *q.shape, device=DEV, dtype=q.dtype)
+    grads = [torch.empty_like(q) for _ in range(3)]
+    cache = [torch.zeros(3, 2, 16, 64, device=DEV, dtype=q.dtype) for _ in range(2)]
+    table, lens = torch.arange(3, dtype=torch.int32, device=DEV)[None], torch.tensor([40], dtype=torch.int32, device=DEV)
+    one = q[:, :, :1].contiguous()
+    bad = [lambda: swa.sink_swa_forward(q, k, v, 9, 2, 0.125, out=q), lambda: swa.sink_swa_forward(q, k, v, 9, 2, 0.125, out=v.view(v.shape)),
+           lambda: swa.sink_swa_backward(q, k, v, o, lse, o, 9, 2, 0.125, out=(grads[0], grads[1], grads[0])),
+           lambda: swa.sink_swa_backward(q, k, v, o, lse, o, 9, 2, 0.125, out=(q, grads[1], grads[2])),
+           lambda: swa.sink_swa_backward(q, k, v, o, lse, o, 9, 2, 0.125, out=(grads[0], both[0], both.view(-1)[64:64 + q.numel()].view_as(q))),
+           lambda: swa.kv_append_rope(None, k, v, None, (), cache[0], cache[0], table, lens),
+           lambda: swa.kv_append_rope(None, cache[0][:1], v[:, :, :16], None, (), *cache, table[:, :1], lens),
+           lambda: swa.sink_swa_decode(one, *cache, table, lens, 9, 2, out=one)]
+    for f in bad:
+        with pytest.raises(ValueError, match="shares memory"):
+            f()
+    # interleaved views of one buffer, as of a fused projection, are fine
+    packed = torch.empty(1, 40, 3, 2, 64, device=DEV, dtype=q.dtype)
+    views = [packed[:, :, i].transpose(1, 2) for i in range(3)]
+    want = swa.sink_swa_backward(q, k, v, o, lse, o, 9, 2, 0.125)
+    for a, b in zip(swa.sink_swa_backward(q, k, v, o, lse, o, 9, 2, 0.125, out=views), want):
+        assert torch.equal(a, b)
+    # autograd learns that an output it had saved was overwritten
+    x = torch.ones_like(q, requires_grad=True)
+    y = torch.empty_like(q)
+    z = (x * y).sum()
+    swa.sink_swa_forward(q, k, v, 9, 2, 0.125, out=y)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+
+
 def test_other_stream():
     case = (1, 2, 1, 400, 100, 4, 64, 64, None)
     t, scale = attn_case(case, BF)
