@@ -19,7 +19,7 @@
 // training step instead of 170).
 //
 // dK/dV of blocks with sinks, which every later query sees, are cut into pieces and joined in order, as in sink_tc_bwd.cuh; rows that
-// end as an infinity or a NaN are done again by the row functions.
+// end as an infinity or a NaN, of a piece too, are done again by the row functions.
 #pragma once
 
 #include "sink_rows.cuh"
@@ -288,6 +288,7 @@ __global__ void __launch_bounds__(kF32Threads, (KIND == 2 && DQ + DV > 128 ? 1 :
   __syncthreads();
   if (threadIdx.x < kF32X) bad_row[threadIdx.x] = 0;
   __syncthreads();
+  const bool near = KIND == 2 && piece >= 0 && piece_near(first, nb, per_head, p.near);         // (rows other than sinks count)
   auto put = [&](auto& v, const View4& t, int dmax, int d, float* part, int i, float f) {
     const int r = ty + kF32Y * i, x = x0 + r;
     float z = 0.f;
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(kF32Threads, (KIND == 2 && DQ + DV > 128 ? 1 :
       if (part) *reinterpret_cast<float4*>(part + (int64_t)r * (a.dqk + a.dv_dim) + col) = o;
       else if (x < a.N) *reinterpret_cast<float4*>((float*)t.ptr + b * t.s0 + h * t.s1 + (int64_t)x * t.s2 + col) = o;
     }
-    if (!part && x < len && !(z == 0.f)) bad_row[r] = 1;
+    if (x < len && (!part || x < a.ns || near) && !(z == 0.f)) bad_row[r] = 1;
   };
   float* part = KIND == 2 && piece >= 0 ? p.part + (((((int64_t)b * a.Hkv + h) * p.n_sb + x0 / kF32X) * p.pieces + piece) * kF32X) * (a.dqk + a.dv_dim) : nullptr;
 #pragma unroll
@@ -324,7 +325,10 @@ __global__ void __launch_bounds__(kF32Threads, (KIND == 2 && DQ + DV > 128 ? 1 :
     if (!bad_row[r]) continue;
     if constexpr (KIND == 0) row_forward<float>(a, b, h, x0 + r, s);
     if constexpr (KIND == 1) row_dq<float>(a, b, h, x0 + r, s);
-    if constexpr (KIND == 2) row_dkdv<float>(a, b, h, x0 + r, s);
+    if constexpr (KIND == 2) {
+      if (part) row_piece<float>(a, b, h, x0 + r, x0, first, nb, per_head, kF32Rows, part + r * (a.dqk + a.dv_dim), 4, s);
+      else row_dkdv<float>(a, b, h, x0 + r, s);
+    }
   }
 }
 

@@ -159,6 +159,24 @@ __device__ __noinline__ void row_dq(const Args& a, int b, int h, int i, float* s
   store_row<T>(a.dq, b, h, i, acc, a.scale, a.dqk, lane);
 }
 
+// Adds what queries lo .. end - 1 of head h give to dk and dv of the key staged in `s`, p_ij (do_i . v_j - delta_i) q_i and p_ij do_i.
+template <typename T>
+__device__ __forceinline__ void add_queries(const Args& a, int b, int h, int lo, int end, const float* s, bool qvec, bool ovec, float* dk, float* dv, int lane) {
+  const int64_t at = ((int64_t)b * a.Hq + h) * a.N;
+  for (int i0 = lo; i0 < end; i0 += 32) {
+    const uint32_t see = __ballot_sync(0xffffffffu, i0 + lane < end);
+    float p = 0.f, ds = 0.f;
+    if (see >> lane & 1u) {
+      p = exp2f(dot_row(s, row_ptr<T>(a.q, b, h, i0 + lane), a.q.s3, a.dqk, qvec) * a.c2 - a.lse[at + i0 + lane]);
+      ds = p * (dot_row(s + kMaxDim, row_ptr<T>(a.d_o, b, h, i0 + lane), a.d_o.s3, a.dv_dim, ovec) - a.delta[at + i0 + lane]);
+    }
+    add_rows(dv, p, see, row_ptr<T>(a.d_o, b, h, i0), a.d_o.s2, a.d_o.s3, a.dv_dim, lane);
+    add_rows(dk, ds, see, row_ptr<T>(a.q, b, h, i0), a.q.s2, a.q.s3, a.dqk, lane);
+  }
+}
+// Behind the last query that sees key j.
+__device__ __forceinline__ int queries_end(const Args& a, int j, int len) { return j < a.ns ? len : (int)min((int64_t)len, (int64_t)j + a.W); }
+
 // dk_j = scale * sum_i p_ij (do_i . v_j - delta_i) q_i,  dv_j = sum_i p_ij do_i, over the heads that share key head hk, in order.
 template <typename T>
 __device__ __noinline__ void row_dkdv(const Args& a, int b, int hk, int j, float* s) {
@@ -170,24 +188,44 @@ __device__ __noinline__ void row_dkdv(const Args& a, int b, int hk, int j, float
     stage_row(s + kMaxDim, row_ptr<T>(a.v, b, hk, j), a.v.s3, a.dv_dim, lane);
     __syncwarp();
     const bool qvec = vec_rows<T>(a.q, a.dqk), ovec = vec_rows<T>(a.d_o, a.dv_dim);
-    const int end = j < a.ns ? len : (int)min((int64_t)len, (int64_t)j + a.W);
-    for (int g = 0; g < a.G; ++g) {
-      const int h = hk * a.G + g;
-      const int64_t at = ((int64_t)b * a.Hq + h) * a.N;
-      for (int i0 = j; i0 < end; i0 += 32) {
-        const uint32_t see = __ballot_sync(0xffffffffu, i0 + lane < end);
-        float p = 0.f, ds = 0.f;
-        if (see >> lane & 1u) {
-          p = exp2f(dot_row(s, row_ptr<T>(a.q, b, h, i0 + lane), a.q.s3, a.dqk, qvec) * a.c2 - a.lse[at + i0 + lane]);
-          ds = p * (dot_row(s + kMaxDim, row_ptr<T>(a.d_o, b, h, i0 + lane), a.d_o.s3, a.dv_dim, ovec) - a.delta[at + i0 + lane]);
-        }
-        add_rows(dv, p, see, row_ptr<T>(a.d_o, b, h, i0), a.d_o.s2, a.d_o.s3, a.dv_dim, lane);
-        add_rows(dk, ds, see, row_ptr<T>(a.q, b, h, i0), a.q.s2, a.q.s3, a.dqk, lane);
-      }
-    }
+    const int end = queries_end(a, j, len);
+    for (int g = 0; g < a.G; ++g) add_queries<T>(a, b, hk * a.G + g, j, end, s, qvec, ovec, dk, dv, lane);
   }
   store_row<T>(a.dk, b, hk, j, dk, a.scale, a.dqk, lane);
   store_row<T>(a.dv, b, hk, j, dv, 1.f, a.dv_dim, lane);
+}
+
+// A piece of a block with sinks, as the tiled kernels cut its stream (cut_pieces): `nb` blocks of `stream` queries, the first of them block `first`
+// of the per_head blocks that every head of the group has from query x0 on.  bad_piece: whether a sum that the kernel left for row j is an
+// infinity or a NaN; row_piece: the row's sums over the piece once more, over the pairs that see each other only.  `part`: the row's place,
+// column c of dK and then dV at c / 4 * s_col4 + c % 4.
+__device__ __forceinline__ bool bad_piece(const Args& a, const float* part, int s_col4, int lane) {
+  bool bad = false;
+  for (int c = lane; c < a.dqk + a.dv_dim; c += 32) bad |= !(fabsf(part[(c >> 2) * s_col4 + (c & 3)]) <= 3.0e38f);
+  return __any_sync(0xffffffffu, bad);
+}
+template <typename T>
+__device__ __noinline__ void row_piece(const Args& a, int b, int hk, int j, int x0, int first, int nb, int per_head, int stream, float* part, int s_col4,
+                                       float* s) {
+  const int lane = threadIdx.x & 31, len = seq_len(a, b);
+  float dk[kDimsPerLane] = {}, dv[kDimsPerLane] = {};
+  __syncwarp();
+  stage_row(s, row_ptr<T>(a.k, b, hk, j), a.k.s3, a.dqk, lane);
+  stage_row(s + kMaxDim, row_ptr<T>(a.v, b, hk, j), a.v.s3, a.dv_dim, lane);
+  __syncwarp();
+  const bool qvec = vec_rows<T>(a.q, a.dqk), ovec = vec_rows<T>(a.d_o, a.dv_dim);
+  const int end = queries_end(a, j, len);
+  for (int n = first; n < first + nb;) {
+    const int g = n / per_head, at = n - g * per_head, blocks = min(per_head - at, first + nb - n);
+    add_queries<T>(a, b, hk * a.G + g, max(j, x0 + at * stream), min(end, x0 + (at + blocks) * stream), s, qvec, ovec, dk, dv, lane);
+    n += blocks;
+  }
+#pragma unroll
+  for (int t = 0; t < kDimsPerLane; ++t) {
+    const int c = lane + 32 * t, e = a.dqk + c;
+    if (c < a.dqk) part[(c >> 2) * s_col4 + (c & 3)] = dk[t];
+    if (c < a.dv_dim) part[(e >> 2) * s_col4 + (e & 3)] = dv[t];
+  }
 }
 
 // KIND 0 forward, 1 dQ, 2 dK/dV.  grid = (rows / 8, heads, B); 8 warps.
@@ -242,10 +280,11 @@ __global__ void __launch_bounds__(256) delta_rows_kernel(const __grid_constant__
 // Every later query sees them: the tiled kernels cut the G * ceil((len - x0) / stream) blocks they stream for such a block of `rows` resident
 // rows into pieces of piece_len, each of which leaves its sums in part [B, Hkv, n_sb, pieces, rows * (d_qk + d_v)], row j and column c of
 // them at j * s_row + c / 4 * s_col4 + c % 4.  Added here in the order of the pieces, one warp per row; a block that is a single piece
-// has gone straight out.
+// has gone straight out.  Sums that are an infinity or a NaN have been done again by the kernel that left them (row_piece), so that nothing
+// is left to repeat here: a row's warps, which have 32 columns each, depend on nothing but the pieces.
 // Pieces of blocks with sinks: as long as an ordinary block's stream (G * near blocks, near = those that rows other than sinks can see), but
-// no more of them than keep every SM busy four times over, or than keep a piece from outlasting the kernels' waits: what they leave
-// for the join stays below 100 MB or so however long the sequences are.
+// no more of them than keep every SM busy four times over, or than keep a piece from outlasting the kernels' waits.  So they are less than
+// twice 592 of `rows` rows together (155 MB of 128 rows of d_qk + d_v = 256) until G * N passes 2^24.
 struct Pieces { int near, len, most; };
 inline Pieces cut_pieces(const Args& a, int n_sb, int rows, int stream) {
   Pieces c;
@@ -275,7 +314,6 @@ struct JoinParams {
 // grid = (rows / 8, Hkv * 8, B): a warp has one row and 32 of its columns (with a warp for all of a row's columns 16384 tokens' 14 pieces took 17 us).
 template <typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) join_kernel(const __grid_constant__ JoinParams p) {
-  __shared__ float smem[kRowWarps][2 * kMaxDim];
   pdl_enter();
   pdl_wait();
   const Args& a = p.a;
@@ -303,10 +341,6 @@ __global__ void __launch_bounds__(32 * kRowWarps) join_kernel(const __grid_const
       for (int e = 0; e < 8; ++e) acc += v[e];
       if (x == 24) break;
     }
-  }
-  if (__any_sync(0xffffffffu, c < d && !(fabsf(acc) <= 3.0e38f))) {               // the whole row again (the row's other warps may do the same)
-    row_dkdv<T>(a, b, hk, j, smem[threadIdx.x >> 5]);
-    return;
   }
   if (c < a.dqk) ((T*)a.dk.ptr)[b * a.dk.s0 + hk * a.dk.s1 + (int64_t)j * a.dk.s2 + c * a.dk.s3] = from_f<T>(acc * a.scale);
   else if (c < d) ((T*)a.dv.ptr)[b * a.dv.s0 + hk * a.dv.s1 + (int64_t)j * a.dv.s2 + (c - a.dqk) * a.dv.s3] = from_f<T>(acc);

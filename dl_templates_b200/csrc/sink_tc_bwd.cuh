@@ -26,7 +26,8 @@
 // Blocks of dK/dV that hold sinks are seen by every later query: their stream is cut into pieces about as long as another block's, the
 // partial sums go to scratch in fp32 and join_kernel (sink_rows.cuh) adds them in order.
 //
-// Infinities and NaN: as in the forward kernel, rows of the result that end as one are done again by row_dq / row_dkdv.
+// Infinities and NaN: as in the forward kernel, rows of the result that end as one are done again by row_dq / row_dkdv, rows of a piece's
+// sums by row_piece.
 #pragma once
 
 #include "sink_tc_common.cuh"
@@ -72,6 +73,11 @@ struct BwdShared {
   int abort_flag, bad;
 };
 static_assert(kItems == 4, "vec is a ring of items too");
+
+// Where a piece leaves its sums: [column / 4][row][4], so that a warp's rows lie side by side.
+__device__ __forceinline__ float* piece_sums(const BwdParams& p, const BwdItem& w) {
+  return p.part + ((((int64_t)w.b * p.a.Hkv + w.h) * p.n_sb + w.x0 / kTile) * p.pieces + w.piece) * (int64_t)kTile * (p.a.dqk + p.a.dv_dim);
+}
 
 template <int KIND, int N>
 __device__ __forceinline__ BwdItem bwd_item(const BwdParams& p, int item) {
@@ -152,6 +158,37 @@ struct BwdWalk {
     }
   }
 };
+
+// Rows of this CTA's items that ended as an infinity or a NaN once more, over the pairs that see each other only; a warp a row.
+template <typename T, int KIND, int N>
+__device__ __noinline__ void bwd_repair(const BwdParams& p, float* s) {
+  const Args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int item = blockIdx.x; item < p.n_items; item += gridDim.x) {
+    const BwdItem w = bwd_item<KIND, N>(p, item);
+    if (!w.nb) continue;
+    const bool near = KIND == 2 && w.piece >= 0 && piece_near(w.first, w.nb, w.per_head, p.near);
+#pragma unroll 1
+    for (int i = w.x0 + warp; i < min(w.len, w.x0 + kTile); i += kThreads / 32) {
+      if (KIND == 2 && w.piece >= 0) {
+        float* part = piece_sums(p, w) + (i - w.x0) * 4;
+        if ((i < a.ns || near) && bad_piece(a, part, 4 * kTile, lane))
+          row_piece<T>(a, w.b, w.h, i, w.x0, w.first, w.nb, w.per_head, N, part, 4 * kTile, s);
+        continue;
+      }
+      bool bad = false;
+      const T* x = row_ptr<T>(KIND == 1 ? a.dq : a.dk, w.b, w.h, i);
+      for (int d = lane; d < a.dqk; d += 32) bad |= !(fabsf(to_f(x[d])) <= 3.0e38f);
+      if constexpr (KIND == 2) {
+        const T* y = row_ptr<T>(a.dv, w.b, w.h, i);
+        for (int d = lane; d < a.dv_dim; d += 32) bad |= !(fabsf(to_f(y[d])) <= 3.0e38f);
+      }
+      if (!__any_sync(0xffffffffu, bad)) continue;
+      if constexpr (KIND == 1) row_dq<T>(a, w.b, w.h, i, s);
+      else row_dkdv<T>(a, w.b, w.h, i, s);
+    }
+  }
+}
 
 template <bool BF16, int KIND, int XC, int VC>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -567,13 +604,14 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
         }
         if (col >= (is_v ? a.dv_dim : a.dqk)) continue;
         if (KIND == 2 && w.piece >= 0) {
-          // sums of a piece: [column / 4][row][4], so that a warp's rows lie side by side
-          float* part = p.part + ((((int64_t)w.b * a.Hkv + w.h) * p.n_sb + w.x0 / kTile) * p.pieces + w.piece) * (int64_t)kTile * (a.dqk + a.dv_dim) +
-                        (int64_t)((is_v ? a.dqk : 0) + col) * kTile + r * 4;
+          float* part = piece_sums(p, w) + (int64_t)((is_v ? a.dqk : 0) + col) * kTile + r * 4;
 #pragma unroll
           for (int u = 0; u < 8; ++u)
-            if (counts && col + 4 * u < (is_v ? a.dv_dim : a.dqk))
+            if (counts && col + 4 * u < (is_v ? a.dv_dim : a.dqk)) {
               *reinterpret_cast<uint4*>(part + u * 4 * kTile) = make_uint4(q[4 * u], q[4 * u + 1], q[4 * u + 2], q[4 * u + 3]);
+#pragma unroll
+              for (int x = 0; x < 4; x += 2) z = f2_fma(f2_pack(__uint_as_float(q[4 * u + x]), __uint_as_float(q[4 * u + x + 1])), 0ull, z);
+            }
         } else if (row0 < a.N) {
           store_columns<BF16>(q, is_v ? 1.f : a.scale, live, z, stg, lane, is_v ? &tm_ov : &tm_oqk, col, is_v ? a.dv_dim : a.dqk, row0, w.h, w.b);
         }
@@ -597,26 +635,7 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (*(volatile int*)&sh->bad && !*(volatile int*)&sh->abort_flag) {
-    float* s = reinterpret_cast<float*>(smem) + warp * 2 * kMaxDim;
-    for (int item = blockIdx.x; item < p.n_items; item += gridDim.x) {
-      const BwdItem w = bwd_item<KIND, N>(p, item);
-      if (!w.nb || w.piece >= 0) continue;
-#pragma unroll 1
-      for (int i = w.x0 + warp; i < min(w.len, w.x0 + kTile); i += kThreads / 32) {
-        bool bad = false;
-        const T* x = row_ptr<T>(KIND == 1 ? a.dq : a.dk, w.b, w.h, i);
-        for (int d = lane; d < a.dqk; d += 32) bad |= !(fabsf(to_f(x[d])) <= 3.0e38f);
-        if constexpr (KIND == 2) {
-          const T* y = row_ptr<T>(a.dv, w.b, w.h, i);
-          for (int d = lane; d < a.dv_dim; d += 32) bad |= !(fabsf(to_f(y[d])) <= 3.0e38f);
-        }
-        if (!__any_sync(0xffffffffu, bad)) continue;
-        if constexpr (KIND == 1) row_dq<T>(a, w.b, w.h, i, s);
-        else row_dkdv<T>(a, w.b, w.h, i, s);
-      }
-    }
-  }
+  if (*(volatile int*)&sh->bad && !*(volatile int*)&sh->abort_flag) bwd_repair<T, KIND, N>(p, reinterpret_cast<float*>(smem) + warp * 2 * kMaxDim);
 }
 
 }  // namespace sink
