@@ -44,14 +44,15 @@ struct F32Shape {
   static constexpr int kSmem = 4 * (kX + kY + kF32X * kF32PPitch);
 };
 
-// 64 rows of a [B, H, N, d] tensor from row `n0` on into rows of `pitch` floats; zeros behind the last row and the last element.
+// ROWS rows of a [B, H, N, d] tensor from row `n0` on into rows of `pitch` floats; zeros behind the sequence's last row and the last element (a weight
+// of zero would make a NaN of what padding may hold).
 template <int ROWS>
-__device__ __forceinline__ void f32_load(float* s, int pitch, int dmax, const View4& t, int b, int h, int n0, int N, int d) {
+__device__ __forceinline__ void f32_load(float* s, int pitch, int dmax, const View4& t, int b, int h, int n0, int len, int d) {
   const float* p = (const float*)t.ptr + b * t.s0 + h * t.s1;
   const int units = dmax / 4;
   for (int x = threadIdx.x; x < ROWS * units; x += kF32Threads) {
     const int r = x / units, c = x % units * 4;
-    const bool on = n0 + r < N && c < d;
+    const bool on = n0 + r < len && c < d;
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(s + r * pitch + c)),
                  "l"(on ? p + (int64_t)(n0 + r) * t.s2 + c : (const float*)t.ptr), "r"(on ? 16 : 0) : "memory");
   }
@@ -169,8 +170,8 @@ __global__ void __launch_bounds__(kF32Threads, (KIND == 2 && DQ + DV > 128 ? 1 :
   const View4 &tq = KIND == 2 ? a.k : a.q, &tv = KIND == 2 ? a.v : a.d_o;          // resident
   const View4 &sq = KIND == 2 ? a.q : a.k, &sv = KIND == 2 ? a.d_o : a.v;          // streamed
   if (nb) {
-    f32_load<kF32X>(xq, S::PQ, DQ, tq, b, h, x0, a.N, a.dqk);
-    if constexpr (KIND != 0) f32_load<kF32X>(xv, S::PV, DV, tv, b, h, x0, a.N, a.dv_dim);
+    f32_load<kF32X>(xq, S::PQ, DQ, tq, b, h, x0, len, a.dqk);
+    if constexpr (KIND != 0) f32_load<kF32X>(xv, S::PV, DV, tv, b, h, x0, len, a.dv_dim);
   }
   // statistics of the resident rows (KIND 0 running, 1 given)
   float m[4], l[4];
@@ -204,8 +205,8 @@ __global__ void __launch_bounds__(kF32Threads, (KIND == 2 && DQ + DV > 128 ? 1 :
       hy = h * a.G + (first + n) / per_head;
     }
     __syncthreads();                                             // the block before has been read
-    f32_load<kF32Rows>(yq, S::PQ, DQ, sq, b, hy, y0, a.N, a.dqk);
-    f32_load<kF32Rows>(yv, S::PV, DV, sv, b, hy, y0, a.N, a.dv_dim);
+    f32_load<kF32Rows>(yq, S::PQ, DQ, sq, b, hy, y0, len, a.dqk);
+    f32_load<kF32Rows>(yv, S::PV, DV, sv, b, hy, y0, len, a.dv_dim);
     asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     float s[4][4];

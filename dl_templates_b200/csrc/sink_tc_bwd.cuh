@@ -27,7 +27,7 @@
 // partial sums go to scratch in fp32 and join_kernel (sink_rows.cuh) adds them in order.
 //
 // Infinities and NaN: as in the forward kernel, rows of the result that end as one are done again by row_dq / row_dkdv, rows of a piece's
-// sums by row_piece.
+// sums by row_piece; padding behind a sequence's end is zeros before it is multiplied.
 #pragma once
 
 #include "sink_tc_common.cuh"
@@ -65,7 +65,7 @@ struct BwdShared {
   // ds_ready: a barrier per score buffer.  Both issuers wait for it, and the second may be behind by a block, waiting for the epilogue; the
   // next phase of a buffer's barrier needs scores that are made only after the products of the one before (s_done).
   uint64_t x_full[2], x_empty[2], y_full[4], y_empty[4], s_full[2], s_done[2], ds_ready[2], dp_full, acc_full, acc_empty, vec_full[4], vec_empty[4],
-      item_full[kItems], item_empty[kItems];
+      item_full[kItems], item_empty[kItems], padded;
   // KIND 2: -lse and -delta of the streamed rows, a ring by blocks; KIND 1: of the resident rows, a ring by items
   alignas(16) float vec[4][2][kTile];
   BwdItem item[kItems];
@@ -251,7 +251,7 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
     if (warp == 0) {
       // ---------------------------------------------------------------- producer
       const uint32_t el = elect_one();
-      int st = 0, par = 1, xb = 0, x_par = 1;
+      int st = 0, par = 1, xb = 0, x_par = 1, pad_par = 0;
       BwdItem w;
       while (take(w)) {
         if (!w.nb) continue;
@@ -269,12 +269,20 @@ sink_bwd_kernel(const __grid_constant__ CUtensorMap tm_xqk, const __grid_constan
           const int row = y.y0, h = y.h;
           wait(&sh->y_empty[st], par);
           if (!ok) break;
-          const uint32_t ys = smem_u32(y_smem) + st * kYStage, ybar = smem_u32(&sh->y_full[st]);
+          const bool pad = holds_padding<N>(row, w.len, a.N);
+          const uint32_t ys = smem_u32(y_smem) + st * kYStage, ybar = smem_u32(pad ? &sh->padded : &sh->y_full[st]);
           mbar_expect_tx_el(el, ybar, kYStage);
 #pragma unroll
           for (int c = 0; c < XC; ++c) tma_load_4d_el(el, ys + c * kY, &tm_yqk, ybar, 64 * c, row, h, w.b);
 #pragma unroll
           for (int c = 0; c < VC; ++c) tma_load_4d_el(el, ys + (XC + c) * kY, &tm_yv, ybar, 64 * c, row, h, w.b);
+          if (pad) {
+            wait(&sh->padded, pad_par);
+            if (!ok) break;
+            pad_par ^= 1;
+            zero_rows<N, XC + VC>(ys, w.len - row, lane);
+            if (lane == 0) mbar_arrive(&sh->y_full[st]);
+          }
           if (++st == p.stages) { st = 0; par ^= 1; }
         }
       }

@@ -28,7 +28,8 @@
 // look (298 us, spills).
 //
 // A hidden pair has P = 0, which is nothing to a sum until the value is an infinity or a NaN: a row that ends as one is done again
-// by row_forward, which touches only what the row sees, after the CTA's last tile.
+// by row_forward, which touches only what the row sees, after the CTA's last tile.  Padding behind a sequence's end costs no row
+// that: it is zeros before it is multiplied (zero_rows).
 //
 // All waits are bounded (umma.cuh); a warp whose wait gave up leaves its loops, the others run into their own limit.
 #pragma once
@@ -59,7 +60,7 @@ struct FwdItem {
 
 struct FwdShared {
   uint64_t q_full, q_empty, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], s_free[2], p_half[2], p_full[2], pv_done[2], o_full[2], o_empty[2],
-      l_full[2], l_empty[2], item_full[kItems], item_empty[kItems];
+      l_full[2], l_empty[2], item_full[kItems], item_empty[kItems], padded;
   FwdItem item[kItems];
   float inv[2][kTile];                          // 1 / l of a tile's rows
   uint32_t tmem_base;
@@ -162,7 +163,7 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     if (warp == 0) {
       // ---------------------------------------------------------------- producer
       const uint32_t el = elect_one();
-      int st = 0, par = 1, q_par = 1;
+      int st = 0, par = 1, q_par = 1, pad_par = 0;
       FwdItem w;
       while (take(w)) {
         if (!w.nb) continue;
@@ -185,10 +186,18 @@ sink_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             tma_load_4d_el(el, smem_u32(k_smem) + st * S::kKStage + c * kB, &tm_k, smem_u32(&sh->k_full[st]), 64 * c, row, w.hk, w.b);
           wait(&sh->v_empty[st], par);
           if (!ok) break;
-          mbar_expect_tx_el(el, smem_u32(&sh->v_full[st]), S::kVStage);
+          const bool pad = holds_padding<N>(row, w.len, a.N);    // (scores of hidden keys are never used, their values are multiplied)
+          const uint32_t vs = smem_u32(v_smem) + st * S::kVStage, vbar = smem_u32(pad ? &sh->padded : &sh->v_full[st]);
+          mbar_expect_tx_el(el, vbar, S::kVStage);
 #pragma unroll
-          for (int c = 0; c < VC; ++c)
-            tma_load_4d_el(el, smem_u32(v_smem) + st * S::kVStage + c * kB, &tm_v, smem_u32(&sh->v_full[st]), 64 * c, row, w.hk, w.b);
+          for (int c = 0; c < VC; ++c) tma_load_4d_el(el, vs + c * kB, &tm_v, vbar, 64 * c, row, w.hk, w.b);
+          if (pad) {
+            wait(&sh->padded, pad_par);
+            if (!ok) break;
+            pad_par ^= 1;
+            zero_rows<N, VC>(vs, w.len - row, lane);
+            if (lane == 0) mbar_arrive(&sh->v_full[st]);
+          }
           if (++st == p.stages) { st = 0; par ^= 1; }
         }
       }

@@ -7,7 +7,7 @@
 
 Layout: ``q [B,Hq,N,d_qk]``, ``k [B,Hkv,N,d_qk]``, ``v [B,Hkv,N,d_v]``, ``o [B,Hq,N,d_v]``; ``Hq`` is a multiple of ``Hkv`` and query head
 ``h`` attends with key head ``h // (Hq // Hkv)``.  ``seq_lens``: ``None`` or int32 ``[B]`` on the device, the tokens of each sequence of a
-padded batch; rows behind a sequence's end are never read as keys, whatever they hold, and their outputs and
+padded batch; rows behind a sequence's end take no part, whatever they hold, and their outputs and
 gradients are zeros.
 
 fp16 / bf16 with head dims up to 128 run on the tensor cores (head dims that are no multiple of 8 are padded with zero columns), everything

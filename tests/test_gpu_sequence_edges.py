@@ -17,6 +17,39 @@ def same_bits(a, b):
     return torch.equal(torch.nan_to_num(a, nan=1e4), torch.nan_to_num(b, nan=1e4)) and torch.equal(torch.isnan(a), torch.isnan(b))
 
 
+# ---- padding -----------------------------------------------------------------------------------------------------------
+# B, Hq, Hkv, N, window, n_sink, d_qk, d_v, lens: ends inside a block, at its first and last row, in the block of the sinks, before it
+PADDED = [
+    (2, 4, 2, 420, 100, 4, 64, 64, [300, 420]),
+    (4, 2, 2, 400, 300, 16, 128, 128, [129, 255, 256, 257]),
+    (2, 4, 1, 700, 90, 40, 128, 128, [651, 30]),            # pieces of the sinks' blocks; an end among the sinks
+    (2, 3, 3, 500, 130, 130, 96, 64, [385, 131]),
+    (1, 4, 2, 520, 200, 3, 64, 128, [401]),
+    (3, 2, 1, 333, 64, 5, 80, 80, [1, 300, 0]),
+    (1, 12, 4, 1500, 512, 16, 80, 80, [1033]),
+]
+
+
+@pytest.mark.parametrize("fill", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype", [F32, F16, BF], ids=["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("case", PADDED, ids=str)
+def test_padding_that_is_not_finite_changes_no_bit(case, dtype, fill):
+    """What lies behind a sequence's end takes no part: results are those of zeros there, bit for bit, so that no row is done a second time
+    for it either."""
+    _, _, _, N, W, ns, _, _, lens = case
+    t, scale = attn_case(case, dtype)
+    for value in (0.0, fill):
+        for b, n in enumerate(lens):
+            for x in NAMES:
+                t[x][b, :, n:] = value
+        got = run_attn(t, lens_tensor(lens), W, ns, scale)
+        if value == 0.0:
+            want = got
+    for n in want:
+        assert bool(torch.isfinite(got[n]).all()) or n == "lse", n
+        assert torch.equal(got[n], want[n]), n
+
+
 # ---- infinities ----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("d, dv", [(128, 128), (64, 64), (64, 128), (96, 40)])
 @pytest.mark.parametrize("dtype", [F32, F16, BF], ids=["fp32", "fp16", "bf16"])
