@@ -225,10 +225,37 @@ void check_sink(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
   TORCH_CHECK_TYPE(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(), "q, k, v must share a dtype");
 }
 
-// 16-bit head dims that are no multiple of 8 reach the tensor-core kernels with zero columns: scores unchanged, zero columns of O.
-int64_t sink_padded(const Tensor& t, int32_t impl) {
-  const int64_t d = t.size(3);
-  return impl != SWA_IMPL_AUTO || t.scalar_type() == at::kFloat || d > 128 ? d : (d + 7) / 8 * 8;
+// The tiled kernels (tensor cores; fp32 on the CUDA cores) want rows that are whole 16-byte units, and up to 128 elements.  What reaches them
+// otherwise is made so here, since the kernels that take anything are a warp a row, tens to hundreds of times slower:
+// head dims are padded with zero columns (scores unchanged, zero columns of O) ...
+int64_t sink_padded(const Tensor& t, const Tensor& q, const Tensor& v, int32_t impl) {
+  const int64_t d = t.size(3), e = t.scalar_type() == at::kFloat ? 4 : 8;
+  return impl != SWA_IMPL_AUTO || q.size(3) > 128 || v.size(3) > 128 ? d : (d + e - 1) / e * e;
+}
+// ... and tensors in other layouts -- an expanded gradient, a view that starts off a 16-byte boundary, odd strides -- are copied.  (Not by
+// contiguous(), which hands a misaligned contiguous tensor back.)
+bool whole_rows(const Tensor& t, int64_t unit = 16) {
+  const int64_t e = unit / t.element_size();
+  if (t.stride(3) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % unit) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) > 1 && (t.stride(i) <= 0 || t.stride(i) % e)) return false;
+  return true;
+}
+Tensor in_whole_rows(const Tensor& t, int64_t unit = 16) { return whole_rows(t, unit) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+// Whether a shape is one of the tiled kernels' (f32_shape and tc_unsupported of the library).
+bool sink_tiles(const Tensor& q, const Tensor& k, const Tensor& v, const SinkWin& w, int32_t impl) {
+  if (q.scalar_type() == at::kFloat) return q.size(3) % 4 == 0 && v.size(3) % 4 == 0 && q.size(3) <= 128 && v.size(3) <= 128;
+  const sink_geom_t g = sink_geom(q, k, v, Tensor(), w, impl);
+  return sink_swa_select(&g) == SWA_IMPL_TC;
+}
+
+// (A dimension of extent 1 may carry any stride.)
+swa_tensor_t sink_view(const Tensor& t) {
+  swa_tensor_t r = view4(t);
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) == 1) r.stride[i] = 0;
+  return r;
 }
 
 Fwd sink_forward(Tensor q, Tensor k, Tensor v, Tensor lens, const SinkWin& w, int32_t impl, Tensor out) {
@@ -240,7 +267,7 @@ Fwd sink_forward(Tensor q, Tensor k, Tensor v, Tensor lens, const SinkWin& w, in
     check_writable(out, "out");
     check_apart(out, {&q, &k, &v}, "out");
   }
-  const int64_t pq = sink_padded(q, impl), pv = sink_padded(v, impl);
+  const int64_t pq = sink_padded(q, q, v, impl), pv = sink_padded(v, q, v, impl);
   if (pq != q.size(3) || pv != v.size(3)) {
     Fwd f = sink_forward(pad_last(q, pq), pad_last(k, pq), pad_last(v, pv), lens, w, impl, Tensor());
     const Tensor o = f.o.narrow(3, 0, v.size(3));
@@ -248,14 +275,16 @@ Fwd sink_forward(Tensor q, Tensor k, Tensor v, Tensor lens, const SinkWin& w, in
     return f;
   }
   const c10::cuda::OptionalCUDAGuard guard(q.device());
-  q = materialise(q); k = materialise(k); v = materialise(v);
+  const bool tiles = sink_tiles(q, k, v, w, impl), direct = out.defined() && (!tiles || whole_rows(out));
+  for (Tensor* t : {&q, &k, &v}) *t = tiles ? in_whole_rows(*t) : materialise(*t);
   Fwd f;
-  f.o = out.defined() ? out : at::empty(shape, q.options());
+  f.o = direct ? out : at::empty(shape, q.options());
   f.lse = new_lse(q);
   const sink_geom_t g = sink_geom(q, k, v, lens, w, impl);
-  const swa_tensor_t tq = view4(q), tk = view4(k), tv = view4(v), to = view4(f.o);
-  if (out.defined()) written(out);
+  const swa_tensor_t tq = sink_view(q), tk = sink_view(k), tv = sink_view(v), to = sink_view(f.o);
+  if (direct) written(out);
   check(sink_swa_fwd(&g, &tq, &tk, &tv, &to, f.lse.data_ptr<float>(), status_ptr(q.get_device()), stream_of(q)), "sink_swa_fwd");
+  if (out.defined() && !direct) f.o = out.copy_(f.o);
   debug_sync();
   return f;
 }
@@ -284,7 +313,7 @@ Grads sink_backward(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor d
     check_apart(out.dk, {&q, &k, &v, &o, &d_o, &lse, &out.dv}, "dk");
     check_apart(out.dv, {&q, &k, &v, &o, &d_o, &lse}, "dv");
   }
-  const int64_t pq = sink_padded(q, impl), pv = sink_padded(v, impl);
+  const int64_t pq = sink_padded(q, q, v, impl), pv = sink_padded(v, q, v, impl);
   if (pq != q.size(3) || pv != v.size(3)) {
     const Grads g = sink_backward(pad_last(q, pq), pad_last(k, pq), pad_last(v, pv), pad_last(o, pv), lse, pad_last(d_o, pv), lens, w, impl, Grads());
     const Tensor dq = g.dq.narrow(3, 0, q.size(3)), dk = g.dk.narrow(3, 0, k.size(3)), dv = g.dv.narrow(3, 0, v.size(3));
@@ -295,19 +324,28 @@ Grads sink_backward(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor d
     return out;
   }
   const c10::cuda::OptionalCUDAGuard guard(q.device());
+  const bool tiles = sink_tiles(q, k, v, w, impl);
   lse = lse.contiguous();
-  q = materialise(q); k = materialise(k); v = materialise(v); o = materialise(o); d_o = materialise(d_o);
-  Grads r = given ? out : Grads{at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options()), at::empty(v.sizes(), v.options())};
+  for (Tensor* t : {&q, &k, &v, &o, &d_o}) *t = tiles ? in_whole_rows(*t) : materialise(*t);
+  auto target = [&](const Tensor& to, const Tensor& like) {
+    const bool direct = to.defined() && (!tiles || whole_rows(to));
+    if (direct) written(to);
+    return direct ? to : at::empty(like.sizes(), like.options());
+  };
+  Grads r{target(out.dq, q), target(out.dk, k), target(out.dv, v)};
   const sink_geom_t g = sink_geom(q, k, v, lens, w, impl);
   const int64_t bytes = sink_swa_bwd_scratch(&g);
   check(bytes < 0 ? (int)bytes : 0, "sink_swa_bwd_scratch");
   const Tensor scratch = at::empty({bytes}, q.options().dtype(at::kByte));
-  const swa_tensor_t tq = view4(q), tk = view4(k), tv = view4(v), to = view4(o), tdo = view4(d_o), tdq = view4(r.dq), tdk = view4(r.dk),
-                     tdv = view4(r.dv);
-  if (given)
-    for (const Tensor* t : {&out.dq, &out.dk, &out.dv}) written(*t);
+  const swa_tensor_t tq = sink_view(q), tk = sink_view(k), tv = sink_view(v), to = sink_view(o), tdo = sink_view(d_o), tdq = sink_view(r.dq),
+                     tdk = sink_view(r.dk), tdv = sink_view(r.dv);
   check(sink_swa_bwd(&g, &tq, &tk, &tv, &to, &tdo, lse.data_ptr<float>(), &tdq, &tdk, &tdv, scratch.data_ptr(), bytes,
                      status_ptr(q.get_device()), stream_of(q)), "sink_swa_bwd");
+  if (given) {
+    if (!r.dq.is_same(out.dq)) r.dq = out.dq.copy_(r.dq);
+    if (!r.dk.is_same(out.dk)) r.dk = out.dk.copy_(r.dk);
+    if (!r.dv.is_same(out.dv)) r.dv = out.dv.copy_(r.dv);
+  }
   debug_sync();
   return r;
 }
@@ -369,7 +407,7 @@ sink_cache_t cache_view(const Tensor& kc, const Tensor& vc, Tensor& table, Tenso
   table = table.contiguous();
   lens = int_vector(lens, B, "seq_lens");
   TORCH_CHECK_VALUE(kc.size(0) <= INT32_MAX && kc.size(2) <= INT32_MAX && table.size(1) <= INT32_MAX, "cache too large");
-  return sink_cache_t{view4(kc), view4(vc), table.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), (int32_t)kc.size(0), (int32_t)kc.size(2),
+  return sink_cache_t{sink_view(kc), sink_view(vc), table.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), (int32_t)kc.size(0), (int32_t)kc.size(2),
                       (int32_t)table.size(1)};
 }
 
@@ -418,7 +456,7 @@ Tensor kv_append(const Tensor& q, const Tensor& k, const Tensor& v, Axes ax, con
   return q_out;
 }
 
-Tensor sink_decode(const Tensor& q, const Tensor& kc, const Tensor& vc, Tensor table, Tensor lens, const SinkWin& w, int32_t impl, Tensor out) {
+Tensor sink_decode(Tensor q, const Tensor& kc, const Tensor& vc, Tensor table, Tensor lens, const SinkWin& w, int32_t impl, Tensor out) {
   poll_status();
   no_gradient({&q, &kc, &vc}, "sink_swa_decode");
   TORCH_CHECK_VALUE(q.dim() == 4 && q.size(2) == 1, "expected q [B,Hq,1,d_qk], one new token of each sequence");
@@ -437,7 +475,9 @@ Tensor sink_decode(const Tensor& q, const Tensor& kc, const Tensor& vc, Tensor t
   } else {
     out = at::empty(shape, q.options());
   }
-  const swa_tensor_t tq = view4(q), to = view4(out);
+  // the split kernel reads pairs of elements of q
+  if (q.size(3) * q.element_size() % 16 == 0 && q.size(3) <= 128) q = in_whole_rows(q, 2 * q.element_size());
+  const swa_tensor_t tq = sink_view(q), to = sink_view(out);
   check(sink_swa_decode(dt, (int32_t)q.size(0), (int32_t)q.size(1), (int32_t)kc.size(1), (int32_t)q.size(3), (int32_t)vc.size(3), w.window,
                         w.n_sink, w.sm, forced_impl(impl), &tq, &c, &to, stream_of(q)), "sink_swa_decode");
   debug_sync();

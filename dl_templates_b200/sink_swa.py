@@ -10,8 +10,9 @@ Layout: ``q [B,Hq,N,d_qk]``, ``k [B,Hkv,N,d_qk]``, ``v [B,Hkv,N,d_v]``, ``o [B,H
 padded batch; rows behind a sequence's end take no part, whatever they hold, and their outputs and
 gradients are zeros.
 
-fp16 / bf16 with head dims up to 128 run on the tensor cores (head dims that are no multiple of 8 are padded with zero columns), everything
-else (fp32, head dims up to 256) on the CUDA cores.  Sums and softmax statistics are fp32; the weights P and dS are rounded to
+fp16 / bf16 with head dims up to 128 run on the tensor cores, fp32 with such head dims in tiles on the CUDA cores; both want rows of whole
+16-byte units, so that other head dims are padded with zero columns and tensors in other layouts (expanded gradients,
+misaligned views) are copied.  Head dims up to 256 run on the CUDA cores, a warp a row.  Sums and softmax statistics are fp32; the weights P and dS are rounded to
 the type of the inputs before the second product.  Results do not depend on the order in which blocks finish.
 """
 from __future__ import annotations

@@ -75,3 +75,89 @@ def test_an_infinity_in_one_piece_of_the_sinks_queries(dtype, d, dv):
     rows = torch.ones(4, N, dtype=torch.bool)
     rows[1, i] = False
     assert inside("dq", (0, rows)) and not torch.isfinite(got["dq"][0, 1, i]).all() and inside("o", (0,))
+
+
+# ---- layouts -----------------------------------------------------------------------------------------------------------
+def off_boundary(x):
+    """The same values, contiguous, one element behind a 16-byte boundary."""
+    y = torch.empty(x.numel() + 16, dtype=x.dtype, device=x.device)[1:1 + x.numel()].view(x.shape)
+    return y.copy_(x)
+
+
+def odd_rows(x):
+    """The same values in rows that are five elements longer."""
+    y = torch.empty(*x.shape[:3], x.shape[3] + 5, dtype=x.dtype, device=x.device)[..., :x.shape[3]]
+    return y.copy_(x)
+
+
+def reversed_dims(x):
+    """The same values with heads and columns the other way round in memory."""
+    return x.permute(3, 2, 0, 1).contiguous().permute(2, 3, 1, 0)
+
+
+LAYOUTS = dict(off_boundary=off_boundary, odd_rows=odd_rows, reversed_dims=reversed_dims)
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF], ids=["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("d, dv", [(64, 64), (128, 80)])
+def test_layouts_of_inputs_and_outputs_change_no_bit(d, dv, dtype, layout):
+    """Inputs or outputs that the tiled kernels cannot read or write in place are copied: the same kernels, the same bits.  One tensor at a
+    time, then all."""
+    f = LAYOUTS[layout]
+    W, ns, lens = 70, 20, lens_tensor([333, 150])
+    t, scale = attn_case((2, 4, 2, 333, W, ns, d, dv, None), dtype)
+    x = {n: t[n].to(DEV) for n in NAMES}
+    o, lse = swa.sink_swa_forward(x["q"], x["k"], x["v"], W, ns, scale, lens)
+    want = swa.sink_swa_backward(x["q"], x["k"], x["v"], o, lse, x["do"], W, ns, scale, lens)
+    for moved in [(n,) for n in (*NAMES, "out")] + [(*NAMES, "out")]:
+        y = {n: f(x[n]) if n in moved else x[n] for n in NAMES}
+        outs = [f(torch.full_like(z, 7.0)) if "out" in moved else torch.full_like(z, 7.0) for z in (o, *want)]
+        o2, lse2 = swa.sink_swa_forward(y["q"], y["k"], y["v"], W, ns, scale, lens, out=outs[0])
+        assert o2.data_ptr() == outs[0].data_ptr() and torch.equal(o2, o) and torch.equal(lse2, lse), moved
+        o_in = f(o) if len(moved) > 1 else o
+        got = swa.sink_swa_backward(y["q"], y["k"], y["v"], o_in, lse, y["do"], W, ns, scale, lens, out=tuple(outs[1:]))
+        for a, b, z in zip(got, want, outs[1:]):
+            assert a.data_ptr() == z.data_ptr() and torch.equal(a, b), moved
+    swa.check_status()
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF], ids=["fp32", "fp16", "bf16"])
+def test_layouts_of_a_decoded_query_change_no_bit(dtype, layout):
+    B, Hq, Hkv, page, n, d = 2, 8, 2, 16, 600, 64
+    g = gen(61)
+    kc, vc = (randn(g, 2 * n // page + 2, Hkv, page, d, dtype=dtype).to(DEV) for _ in range(2))
+    q = randn(g, B, Hq, 1, d, dtype=dtype).to(DEV)
+    table = torch.arange(2 * (n // page + 1), dtype=torch.int32, device=DEV).view(B, -1)
+    lens = lens_tensor([n, n - 77])
+    want = swa.sink_swa_decode(q, kc, vc, table, lens, 400, 4, 0.125)
+    out = LAYOUTS[layout](torch.full_like(q, 7.0))
+    got = swa.sink_swa_decode(LAYOUTS[layout](q), kc, vc, table, lens, 400, 4, 0.125, out=out)
+    assert got.data_ptr() == out.data_ptr() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["fp32", "bf16"])
+def test_gradient_of_a_sum_is_that_of_its_contiguous_copy(dtype):
+    """o.sum() hands an expanded gradient on, all of whose strides are 0."""
+    t, scale = attn_case((2, 4, 2, 500, 90, 4, 64, 64, None), dtype)
+    x = [t[n].to(DEV).requires_grad_() for n in ("q", "k", "v")]
+    want = torch.autograd.grad(swa.SinkSwa.apply(*x, None, 90, 4, scale), x, torch.ones_like(t["do"]).to(DEV))
+    got = torch.autograd.grad(swa.SinkSwa.apply(*x, None, 90, 4, scale).sum(), x)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("d, dv", [(37, 21), (64, 90), (126, 128)])
+def test_fp32_head_dims_that_fill_no_unit_are_padded(d, dv):
+    """fp32 heads that are no multiple of 4: the tiled kernels' results with zero columns, bit for bit, and right."""
+    case = (2, 4, 2, 300, 80, 6, d, dv, [300, 177])
+    t, scale = attn_case(case, F32)
+    pad = lambda z, n: torch.nn.functional.pad(z, (0, n - z.shape[3]))
+    up = lambda n: (n + 3) // 4 * 4
+    p = dict(q=pad(t["q"], up(d)), k=pad(t["k"], up(d)), v=pad(t["v"], up(dv)), do=pad(t["do"], up(dv)))
+    want, got = (run_attn(z, lens_tensor(case[-1]), 80, 6, scale) for z in (p, t))
+    val, bound = orc.attention(t["q"], t["k"], t["v"], case[-1], 80, 6, scale, t["do"])
+    for n in got:
+        assert torch.equal(got[n], want[n][..., :got[n].shape[-1]] if n != "lse" else want[n]), n
+        orc.check(got[n], val[n], bound[n], n)
