@@ -405,25 +405,22 @@ int sink_swa_fwd(const sink_geom_t* g, const swa_tensor_t* q, const swa_tensor_t
   return launch_rows<0>(a, g->dtype, st);
 }
 
-// The softmax delta: rows of whole 16-byte units here, others by the kernels for grids (a sequence is a grid of one column).
+// The softmax delta: rows of whole 16-byte units, up to 32 of them, or any others.
 static int launch_delta(const swa::sink::Args& a, const sink_geom_t* g, const swa_tensor_t* o, const swa_tensor_t* d_o, void* stream) {
   const int e = g->dtype == SWA_F32 ? 4 : 8, units = g->d_v / e;
   auto whole = [&](const swa_tensor_t* t) {
     return t->stride[3] == 1 && (uintptr_t)t->ptr % 16 == 0 && t->stride[0] % e == 0 && t->stride[1] % e == 0 && t->stride[2] % e == 0;
   };
+  cudaError_t err = cudaSuccess;
   if (g->d_v % e || units > 32 || !whole(o) || !whole(d_o)) {
-    if ((int64_t)g->B * g->Hq > 65535) return fail(E_SHAPE, "B*Hq exceeds 65535");
-    swa_geom_t sg;
-    memset(&sg, 0, sizeof(sg));
-    sg.dtype = g->dtype; sg.B = g->B; sg.H = g->Hq; sg.b_size = 1; sg.t_height = g->N; sg.t_width = 1; sg.d_qk = g->d_qk; sg.d_v = g->d_v;
-    sg.sm_scale = g->sm_scale;
-    return swa_bwd_delta(&sg, o, d_o, a.delta, stream);
+    const dim3 grid((a.N + swa::sink::kRowWarps - 1) / swa::sink::kRowWarps, a.Hq, a.B);
+    SINK_DISPATCH(g->dtype, err = swa::launch_stream(swa::sink::delta_any_kernel<T>, grid, 32 * swa::sink::kRowWarps, (cudaStream_t)stream, a));
+    return launched(err, "sink delta");
   }
   int group = 1;
   while (group < units) group *= 2;
   const int rows = 256 / group * swa::sink::kDeltaRows;
   const dim3 grid((a.N + rows - 1) / rows, a.Hq, a.B);
-  cudaError_t err = cudaSuccess;
   SINK_DISPATCH(g->dtype, err = swa::launch_stream(swa::sink::delta_rows_kernel<T>, grid, 256, (cudaStream_t)stream, a, units, group));
   return launched(err, "sink delta");
 }

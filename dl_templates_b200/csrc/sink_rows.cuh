@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
 
 // ---- delta = sum of o * do -----------------------------------------------------------------------------------------------
 // Rows of whole 16-byte units: `group` lanes (the power of two that holds a row's units) take kDeltaRows rows, whose loads are in flight
-// together (72000 rows of 80 16-bit elements: 8.7 us; a row at a time, as for grids, 11.9).  Rows behind a sequence's end are left out.
+// together (72000 rows of 80 16-bit elements: 8.7 us; a row at a time 11.9).  Rows behind a sequence's end are left out.
 constexpr int kDeltaRows = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) delta_rows_kernel(const __grid_constant__ Args a, int units, int group) {
@@ -274,6 +274,20 @@ __global__ void __launch_bounds__(256) delta_rows_kernel(const __grid_constant__
     const int n = n0 + r * per_block;
     if (part == 0 && n < len) a.delta[((int64_t)b * a.Hq + h) * a.N + n] = acc;
   }
+}
+
+// Any type, stride and head dim: a warp a row.  grid = (rows / 8, Hq, B).
+template <typename T>
+__global__ void __launch_bounds__(32 * kRowWarps) delta_any_kernel(const __grid_constant__ Args a) {
+  pdl_enter();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, n = blockIdx.x * kRowWarps + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
+  if (n >= seq_len(a, b)) return;
+  const T *x = row_ptr<T>(a.o, b, h, n), *y = row_ptr<T>(a.d_o, b, h, n);
+  float acc = 0.f;
+  for (int d = lane; d < a.dv_dim; d += 32) acc = fmaf(to_f(x[d * a.o.s3]), to_f(y[d * a.d_o.s3]), acc);
+  acc = lanes_sum(acc);
+  if (lane == 0) a.delta[((int64_t)b * a.Hq + h) * a.N + n] = acc;
 }
 
 // ---- dK and dV of blocks with sinks --------------------------------------------------------------------------------------

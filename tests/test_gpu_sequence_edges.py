@@ -161,3 +161,22 @@ def test_fp32_head_dims_that_fill_no_unit_are_padded(d, dv):
     for n in got:
         assert torch.equal(got[n], want[n][..., :got[n].shape[-1]] if n != "lse" else want[n]), n
         orc.check(got[n], val[n], bound[n], n)
+
+
+# ---- many heads --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype, dv", [(F32, 132), (F32, 18), (F16, 9)], ids=str)
+def test_backward_takes_as_many_heads_as_forward(dtype, dv):
+    """More than 65535 heads in a batch, in layouts for every delta kernel: the gradients of each half of the batch."""
+    B, H, Hkv, N, d = 2, 33000, 1000, 3, 4
+    g = gen(B, H, dv)
+    q, k, v, do = (randn(g, B, h, N, n, dtype=dtype).to(DEV) for h, n in ((H, d), (Hkv, d), (Hkv, dv), (H, dv)))
+    for f in (lambda z: z, reversed_dims):
+        for impl in ("auto", "simt"):
+            o, lse = swa.sink_swa_forward(q, k, v, 2, 1, 0.5, impl=impl)
+            got = swa.sink_swa_backward(q, k, v, o, lse, f(do), 2, 1, 0.5, impl=impl)
+            for b in range(B):
+                s = slice(b, b + 1)
+                want = swa.sink_swa_backward(q[s], k[s], v[s], o[s], lse[s], f(do[s]), 2, 1, 0.5, impl=impl)
+                for a, z in zip(got, want):
+                    assert torch.equal(a[s], z)
+    swa.check_status()
