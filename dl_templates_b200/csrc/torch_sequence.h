@@ -48,17 +48,12 @@ void written(const Tensor& t) {
   if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-bool capturing(const c10::Stream& s) {
-  const cudaStream_t stream = c10::cuda::CUDAStream(s).stream();
-  if (!stream) return false;                                     // the default stream never is
-  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-  C10_CUDA_CHECK(cudaStreamIsCapturing(stream, &st));
-  return st != cudaStreamCaptureStatusNone;
-}
+bool legacy_default(const c10::Stream& s) { return c10::cuda::CUDAStream(s).stream() == nullptr; }
 
-// While a graph is captured, autograd's engine would record events on the stream that an older graph's leaf accumulators live on,
-// which is not part of the capture; what follows ends the process inside the engine.  Refused here, while nothing has been launched:
-// for every leaf that the inputs come from, since all of them take part in the backward pass.
+// While a graph is captured, autograd's engine has the stream of each leaf's accumulator wait for the captured one and then waits for it in turn.
+// A side stream -- a warm-up's, whose last loss is still there -- becomes a part of the capture by that and leaves it again.  The legacy default
+// stream may take no part in a capture: what follows ends the process inside the engine.  Refused here, while nothing has been
+// launched: for every leaf that the inputs come from, since all of them take part in the backward pass.
 void check_capture(std::initializer_list<const Tensor*> inputs) {
   for (const Tensor* t : inputs)
     if (!t->is_cuda()) return;                                   // (refused further on)
@@ -78,9 +73,10 @@ void check_capture(std::initializer_list<const Tensor*> inputs) {
       if (e.function) todo.push_back(e.function);
     if (!dynamic_cast<const torch::autograd::AccumulateGrad*>(n.get())) continue;
     const std::optional<c10::Stream> s = n->stream();
-    TORCH_CHECK(!s.has_value() || capturing(*s),
-                "a leaf of this call belongs to an autograd graph recorded on another stream that is still alive; its backward pass "
-                "cannot be captured: drop that graph (its outputs and losses) before capturing, or capture with detached leaves");
+    TORCH_CHECK(!s.has_value() || !legacy_default(*s),
+                "a leaf of this call belongs to an autograd graph recorded on the default stream that is still alive; its backward pass "
+                "cannot be captured: drop that graph (its outputs and losses) before capturing, record it on a side stream, or capture with "
+                "detached leaves");
   }
 }
 

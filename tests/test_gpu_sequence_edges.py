@@ -180,3 +180,39 @@ def test_backward_takes_as_many_heads_as_forward(dtype, dv):
                 for a, z in zip(got, want):
                     assert torch.equal(a[s], z)
     swa.check_status()
+
+
+# ---- captures ----------------------------------------------------------------------------------------------------------
+def test_a_whole_step_is_captured_after_a_warm_up_on_a_side_stream():
+    """The usual recipe: some steps on a side stream, whose last loss (and with it the leaves' accumulators of that stream) stays alive, then the
+    same step captured and replayed."""
+    g = gen(31)
+    N, W, ns = 200, 50, 4
+    w = randn(g, 1, 2, N, 64).to(DEV).requires_grad_()
+    k, v, do = (randn(g, 1, 2, N, 64).to(DEV) for _ in range(3))
+    rope = swa.RotaryPositionEncodingAxes((32,), (N,)).to(DEV)
+    pos = torch.arange(N, dtype=torch.int32, device=DEV)[None]
+
+    def loss_of():
+        qr, kr = rope(w * 2, k, pos)
+        return (swa.SinkSwa.apply(qr, kr, v, None, W, ns, 0.125).float() * do.float()).sum()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(3):
+            w.grad = None
+            loss = loss_of()
+            loss.backward()
+    torch.cuda.current_stream().wait_stream(s)
+    want = w.grad.clone()
+    w.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = loss_of()
+        captured.backward()
+    w.grad.fill_(float("nan"))
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(w.grad, want) and torch.equal(captured.detach(), loss.detach())
+    swa.check_status()
