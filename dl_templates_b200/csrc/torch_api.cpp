@@ -911,10 +911,13 @@ PyMethodDef g_methods[] = {SWA_DEF("tiled_swa", py_tiled_swa),
                            SWA_DEF("check_status", py_check_status),
                            SWA_DEF("poll_status", py_poll_status),
                            SWA_DEF("rope_axes", py_rope_axes),
-                           SWA_DEF("rope_axes_to", py_rope_axes_to),
+                           SWA_DEF("rope_axes_to", py_rope_axes_to<false>),
+                           SWA_DEF("rope_axes_to_body", py_rope_axes_to<true>),
                            SWA_DEF("sink_swa", py_sink_swa),
-                           SWA_DEF("sink_forward", py_sink_forward),
-                           SWA_DEF("sink_backward", py_sink_backward),
+                           SWA_DEF("sink_forward", py_sink_forward<false>),
+                           SWA_DEF("sink_forward_body", py_sink_forward<true>),
+                           SWA_DEF("sink_backward", py_sink_backward<false>),
+                           SWA_DEF("sink_backward_body", py_sink_backward<true>),
                            SWA_DEF("kv_append", py_kv_append),
                            SWA_DEF("sink_decode", py_sink_decode),
                            SWA_DEF("set_general_sequence", py_set_general_sequence),

@@ -80,6 +80,14 @@ void check_capture(std::initializer_list<const Tensor*> inputs) {
   }
 }
 
+// What the entries without an autograd.Function cannot answer and would drop without a word: a tangent of an input, and the call itself in a
+// trace, which would hold its output as torch found it, empty.
+void nothing_to_record(std::initializer_list<const Tensor*> inputs, const char* name) {
+  TORCH_CHECK(!at::tracer::impl::is_dispatch_enabled(), name, " leaves nothing in a jit trace: trace SinkSwa.apply or RotaryPEAxes.apply");
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), name, " has no forward-mode derivative: an input carries a tangent");
+}
+
 // What a backward node does first: its gradients are no functions of the graph.
 void no_second_derivative(const char* name) {
   TORCH_CHECK(!c10::GradMode::is_enabled(), name, " has no second derivatives: call backward without create_graph");
@@ -527,7 +535,10 @@ PyObject* py_rope_axes(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return pack({y[0], y[1]});
   });
 }
+// The entries below come twice where an autograd.Function is made of them: BODY is what its forward and backward call, which torch has
+// asked for tangents and recorded in a trace itself.
 // rope_axes_to(x, positions, tables, inverse) -> rotated copy
+template <bool BODY>
 PyObject* py_rope_axes_to(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Args a{args, n};
@@ -535,6 +546,10 @@ PyObject* py_rope_axes_to(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Axes ax = axes_args(a);
     const bool inverse = a.i32() != 0;
     a.done();
+    if (!BODY) {
+      nothing_to_record({&x}, "rope_axes_apply_to");
+      for (const Tensor& t : ax.tables) nothing_to_record({&t}, "rope_axes_apply_to");
+    }
     const at::AutoGradMode no_grad(false);
     return THPVariable_Wrap(without_gil([&] { return rotate_axes(x, Tensor(), ax, inverse)[0]; }));
   });
@@ -551,6 +566,7 @@ PyObject* py_sink_swa(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 // sink_forward(q, k, v, seq_lens, window, n_sink, sm_scale, impl, out) -> (o, lse)
+template <bool BODY>
 PyObject* py_sink_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Args a{args, n};
@@ -559,12 +575,14 @@ PyObject* py_sink_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int32_t impl = a.i32();
     const Tensor out = a.maybe_tensor();
     a.done();
+    if (!BODY) nothing_to_record({&q, &k, &v, &out}, "sink_swa_forward");
     const at::AutoGradMode no_grad(false);
     const Fwd f = without_gil([&] { return sink_forward(q, k, v, lens, w, impl, out); });
     return pack({f.o, f.lse});
   });
 }
 // sink_backward(q, k, v, o, lse, do, seq_lens, window, n_sink, sm_scale, impl, dq, dk, dv) -> (dq, dk, dv)
+template <bool BODY>
 PyObject* py_sink_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Args a{args, n};
@@ -573,6 +591,7 @@ PyObject* py_sink_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int32_t impl = a.i32();
     const Grads out{a.maybe_tensor(), a.maybe_tensor(), a.maybe_tensor()};
     a.done();
+    if (!BODY) nothing_to_record({&q, &k, &v, &o, &lse, &d_o, &out.dq, &out.dk, &out.dv}, "sink_swa_backward");
     const at::AutoGradMode no_grad(false);
     const Grads g = without_gil([&] { return sink_backward(q, k, v, o, lse, d_o, lens, w, impl, out); });
     return pack({g.dq, g.dk, g.dv});
@@ -586,6 +605,8 @@ PyObject* py_kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Axes ax = axes_args(a);
     const Tensor kc = a.tensor(), vc = a.tensor(), table = a.tensor(), lens = a.tensor(), fresh = a.maybe_tensor();
     a.done();
+    nothing_to_record({&q, &k, &v, &kc, &vc}, "kv_append_rope");
+    for (const Tensor& t : ax.tables) nothing_to_record({&t}, "kv_append_rope");
     const Tensor y = without_gil([&] { return kv_append(q, k, v, ax, kc, vc, table, lens, fresh); });
     if (!y.defined()) Py_RETURN_NONE;
     return THPVariable_Wrap(y);
@@ -600,6 +621,7 @@ PyObject* py_sink_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int32_t impl = a.i32();
     const Tensor out = a.maybe_tensor();
     a.done();
+    nothing_to_record({&q, &kc, &vc, &out}, "sink_swa_decode");
     return THPVariable_Wrap(without_gil([&] { return sink_decode(q, kc, vc, table, lens, w, impl, out); }));
   });
 }

@@ -11,7 +11,7 @@ while they change.  A page number outside the cache is no page -- nothing is wri
 pages that neither the window nor the sinks reach can be given back and their entries set to -1.
 
 Two new tokens of one call never share a slot: the pages they fall into belong to one sequence each (a page that several sequences
-read, a shared prefix, may stand in all their tables).  Neither call records gradients.
+read, a shared prefix, may stand in all their tables).  Neither call records gradients, tangents or a jit trace: inputs that ask for one are refused.
 """
 from __future__ import annotations
 

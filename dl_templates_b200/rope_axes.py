@@ -20,8 +20,9 @@ from .sink_swa import SinkSwa
 
 
 def rope_axes_apply_to(x: torch.Tensor, positions: torch.Tensor, tables, inverse: bool = False) -> torch.Tensor:
-    """The rotation (or its inverse) of ``x [B,H,N,C]`` in a new contiguous tensor.  ``positions``: int32 ``[axes, N]`` or
-    ``[B, axes, N]``; ``tables``: one fp32 ``[max_position, pairs, 2]`` (cos, sin) table per axis (``make_cs_table``)."""
+    """The rotation (or its inverse) of ``x [B,H,N,C]`` in a new contiguous tensor; no autograd graph (tangents and jit traces are
+    refused).  ``positions``: int32 ``[axes, N]`` or ``[B, axes, N]``; ``tables``: one fp32 ``[max_position, pairs, 2]`` (cos, sin)
+    table per axis (``make_cs_table``)."""
     return _native.rope_axes_to(x, positions, tables, int(inverse))
 
 
@@ -35,13 +36,13 @@ class RotaryPEAxes(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, *tables):
         ctx.save_for_backward(positions, *tables)
-        return rope_axes_apply_to(q, positions, tables), rope_axes_apply_to(k, positions, tables)
+        return _native.rope_axes_to_body(q, positions, tables, 0), _native.rope_axes_to_body(k, positions, tables, 0)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         positions, *tables = ctx.saved_tensors
-        return (rope_axes_apply_to(dq, positions, tables, True), rope_axes_apply_to(dk, positions, tables, True), None,
+        return (_native.rope_axes_to_body(dq, positions, tables, 1), _native.rope_axes_to_body(dk, positions, tables, 1), None,
                 *(None,) * len(tables))
 
 

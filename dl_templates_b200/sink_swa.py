@@ -28,7 +28,7 @@ MAX_SINKS = 1024                    # SINK_MAX_SINKS of include/swa_sequence.h
 
 
 def sink_swa_forward(q, k, v, window, n_sink, sm_scale, seq_lens=None, impl="auto", out=None):
-    """Returns ``(o, lse)``, ``lse`` fp32 ``[B,Hq,N]`` in the base-2 domain (``-inf`` for rows behind a sequence's end).  ``out``: an
+    """No autograd graph (tangents and jit traces are refused).  Returns ``(o, lse)``, ``lse`` fp32 ``[B,Hq,N]`` in the base-2 domain (``-inf`` for rows behind a sequence's end).  ``out``: an
     optional ``[B,Hq,N,d_v]`` tensor or strided view that O is written into; it shares no memory with the inputs."""
     return _native.sink_forward(q, k, v, seq_lens, window, n_sink, sm_scale, _lib.impl_code(impl), out)
 
@@ -63,7 +63,7 @@ class SinkSwa(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, seq_lens, *win):
-        o, lse = sink_swa_forward(q, k, v, *win, seq_lens)
+        o, lse = _native.sink_forward_body(q, k, v, seq_lens, *win, _lib.IMPL_AUTO, None)
         ctx.save_for_backward(q, k, v, lse, o, *(() if seq_lens is None else (seq_lens,)))
         ctx.win = win
         return o
@@ -72,4 +72,4 @@ class SinkSwa(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
         q, k, v, lse, o, *lens = ctx.saved_tensors
-        return (*sink_swa_backward(q, k, v, o, lse, do, *ctx.win, lens[0] if lens else None), *(None,) * 4)
+        return (*_native.sink_backward_body(q, k, v, o, lse, do, lens[0] if lens else None, *ctx.win, _lib.IMPL_AUTO, None, None, None), *(None,) * 4)

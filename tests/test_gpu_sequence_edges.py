@@ -216,3 +216,36 @@ def test_a_whole_step_is_captured_after_a_warm_up_on_a_side_stream():
     torch.cuda.synchronize()
     assert torch.equal(w.grad, want) and torch.equal(captured.detach(), loss.detach())
     swa.check_status()
+
+
+# ---- entries without an autograd.Function ------------------------------------------------------------------------------
+def raw_entries():
+    g = gen(41)
+    q, k, v = (randn(g, 1, 2, 40, 64).to(DEV) for _ in range(3))
+    one = q[:, :, :1].contiguous()
+    o, lse = swa.sink_swa_forward(q, k, v, 9, 2, 0.125)
+    pos, tab = torch.zeros(1, 40, dtype=torch.int32, device=DEV), swa.make_cs_table(16, 8, device=DEV)
+    kc, vc = (torch.zeros(3, 2, 16, 64, device=DEV, dtype=BF) for _ in range(2))
+    table, lens = torch.arange(3, dtype=torch.int32, device=DEV)[None], torch.tensor([40], dtype=torch.int32, device=DEV)
+    return {"sink_swa_fwd": (lambda x: swa.sink_swa_fwd(x, k, v, 9, 2, 0.125), q),
+            "sink_swa_forward": (lambda x: swa.sink_swa_forward(q, x, v, 9, 2, 0.125)[0], k),
+            "sink_swa_backward": (lambda x: swa.sink_swa_backward(q, k, v, o, lse, x, 9, 2, 0.125)[0], o),
+            "rope_axes_apply_to": (lambda x: swa.rope_axes_apply_to(x, pos, (tab,)), q),
+            "kv_append_rope": (lambda x: swa.kv_append_rope(x, k, v, None, None, kc, vc, table, lens), q),
+            "sink_swa_decode": (lambda x: swa.sink_swa_decode(x, kc, vc, table, lens, 9, 2), one)}
+
+
+@pytest.mark.parametrize("entry", ["sink_swa_fwd", "sink_swa_forward", "sink_swa_backward", "rope_axes_apply_to", "kv_append_rope", "sink_swa_decode"])
+def test_entries_that_record_nothing_refuse_tangents_and_traces(entry):
+    """A tangent would be dropped without a word, and a trace would hold an empty output and not the call."""
+    import torch.autograd.forward_ad as fwAD
+    f, x = raw_entries()[entry]
+    with torch.no_grad():
+        want = f(x).clone()
+        with fwAD.dual_level():
+            with pytest.raises(RuntimeError, match="tangent"):
+                f(fwAD.make_dual(x, torch.ones_like(x)))
+            assert torch.equal(f(x), want)                       # others go on
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(f, (x,), check_trace=False)
+        assert torch.equal(f(x), want)
