@@ -249,3 +249,211 @@ def test_entries_that_record_nothing_refuse_tangents_and_traces(entry):
         with pytest.raises(RuntimeError, match="trace"):
             torch.jit.trace(f, (x,), check_trace=False)
         assert torch.equal(f(x), want)
+
+
+# ---- as torch's autograd sees them ---------------------------------------------------------------------------------------
+def functions():
+    g = gen(43)
+    q, k, v = randn(g, 2, 4, 90, 64).to(DEV), randn(g, 2, 2, 90, 64).to(DEV), randn(g, 2, 2, 90, 64).to(DEV)
+    pos, tab = torch.arange(90, dtype=torch.int32, device=DEV)[None], swa.make_cs_table(16, 90, device=DEV)
+    lens = lens_tensor([90, 51])
+    return {"sink": lambda a, b, c: swa.SinkSwa.apply(a, b, c, lens, 30, 4, 0.125),
+            "rope": lambda a, b, c: torch.cat(swa.RotaryPEAxes.apply(a, b, pos, tab), 1)}, (q, k, v)
+
+
+@pytest.mark.parametrize("entry", ["sink", "rope"])
+def test_forward_mode_and_functorch_are_refused(entry):
+    import torch.autograd.forward_ad as fwAD
+    fs, (q, k, v) = functions()
+    f = fs[entry]
+    for grad_mode in (True, False):
+        with torch.set_grad_enabled(grad_mode), fwAD.dual_level():
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                f(fwAD.make_dual(q, torch.ones_like(q)), k, v)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda x: f(x, k, v), (q,), (torch.ones_like(q),))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: f(x, k, v).float().sum())(q)
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda x: f(x, k, v))(torch.stack([q, q]))
+
+
+@pytest.mark.parametrize("entry", ["sink", "rope"])
+def test_a_trace_holds_the_call_and_not_its_result(entry):
+    fs, (q, k, v) = functions()
+    f = fs[entry]
+    with torch.no_grad():
+        traced = torch.jit.trace(f, (q, k, v), check_trace=False)
+        assert torch.equal(traced(q * 2, k * 3, v + 1), f(q * 2, k * 3, v + 1))
+
+
+@pytest.mark.parametrize("entry", ["sink", "rope"])
+def test_saved_tensor_hooks_and_checkpointing(entry):
+    from torch.utils.checkpoint import checkpoint
+    fs, ins = functions()
+    f = fs[entry]
+    ins = ins if entry == "sink" else ins[:2]
+    call = f if entry == "sink" else lambda a, b: f(a, b, None)
+    res = []
+    for wrap in (lambda *t: call(*t), lambda *t: checkpoint(call, *t, use_reentrant=False), lambda *t: checkpoint(call, *t, use_reentrant=True)):
+        t = [x.clone().requires_grad_(True) for x in ins]
+        o = wrap(*t)
+        o.float().square().sum().backward()
+        res.append([o.detach(), *(x.grad for x in t)])
+    packs = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: (packs.append(1), x.cpu())[1], lambda x: x.to(DEV)):
+        t = [x.clone().requires_grad_(True) for x in ins]
+        o = call(*t)
+    o.float().square().sum().backward()
+    res.append([o.detach(), *(x.grad for x in t)])
+    assert len(packs) >= 2
+    for r in res[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, res[0]))
+
+
+# ---- threads, streams ----------------------------------------------------------------------------------------------------
+def attn_step(t, lens, W, ns, scale):
+    x = [t[n].detach().requires_grad_(True) for n in ("q", "k", "v")]
+    pos = torch.arange(t["q"].shape[2], dtype=torch.int32, device=DEV)[None]
+    tab = swa.make_cs_table(4, 64, device=DEV)
+    qr, kr = swa.RotaryPEAxes.apply(x[0], x[1], pos, tab)
+    o = swa.SinkSwa.apply(qr, kr, x[2], lens, W, ns, scale)
+    return (o.detach(), *torch.autograd.grad(o, x, t["do"]))
+
+
+def test_two_threads_on_two_streams():
+    import threading
+    cases = []
+    for c, dtype in (((2, 4, 2, 400, 100, 16, 64, 64, [400, 333]), BF), ((1, 2, 1, 500, 60, 130, 128, 128, None), F16),
+                     ((1, 4, 4, 210, 50, 4, 32, 32, [200]), F32), ((1, 3, 3, 300, 128, 5, 96, 64, None), BF)):
+        t, scale = attn_case(c, dtype)
+        cases.append(({n: z.to(DEV) for n, z in t.items()}, lens_tensor(c[-1]), c[4], c[5], scale))
+    torch.cuda.synchronize()
+    results, errors = [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for r in range(10):
+                    for j in range(len(cases)):
+                        c = (j * (2 * i + 1) + r) % len(cases)
+                        results[i].append((c, attn_step(*cases[c])))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                               # noqa: BLE001 (shown by the assertion below)
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors
+    torch.cuda.synchronize()
+    swa.check_status()
+    want = [attn_step(*c) for c in cases]
+    for per_thread in results:
+        assert len(per_thread) == 40
+        for c, got in per_thread:
+            assert all(torch.equal(a, b) for a, b in zip(got, want[c]))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_kernels_started_early_between_foreign_ones(dtype):
+    """Products write the inputs right before the calls, and they are overwritten right after: training step, then append and decode."""
+    W, ns = 90, 4
+    sets = []
+    for s in range(3):
+        g = gen(51, s)
+        sets.append({n: randn(g, 1, h, 700, 64, dtype=dtype).to(DEV) for n, h in (("q", 4), ("k", 2), ("v", 2), ("do", 4))})
+    eye = torch.eye(64, device=DEV, dtype=dtype)
+    kc, vc = (torch.zeros(12, 2, 64, 64, device=DEV, dtype=dtype) for _ in range(2))
+    table, lens = torch.arange(12, dtype=torch.int32, device=DEV)[None], torch.tensor([700], dtype=torch.int32, device=DEV)
+    live = {n: torch.empty_like(x) for n, x in sets[0].items()}
+
+    def sequence(src):
+        for n in live:
+            torch.matmul(src[n], eye, out=live[n])
+        got = attn_step(live, None, W, ns, 0.125)
+        swa.kv_append_rope(None, live["k"], live["v"], None, None, kc, vc, table, lens)
+        o = swa.sink_swa_decode(live["q"][:, :, -1:], kc, vc, table, lens, W, ns, 0.125)
+        for x in (*live.values(), kc, vc):
+            x.fill_(float("nan"))
+        return (*got, o)
+    prev = torch.backends.cuda.matmul.allow_tf32
+    torch.backends.cuda.matmul.allow_tf32 = False
+    try:
+        want = []
+        for s in sets:
+            want.append([x.clone() for x in sequence(s)])
+            torch.cuda.synchronize()
+        with torch.cuda.stream(torch.cuda.Stream()):
+            runs = [[sequence(s) for s in sets] for _ in range(4)]
+            torch.cuda.current_stream().synchronize()
+    finally:
+        torch.backends.cuda.matmul.allow_tf32 = prev
+    for got in runs:
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert all(bool(torch.isfinite(x).all()) for x in want[0])
+    swa.check_status()
+
+
+# ---- widths of the blocks of sinks, wide heads ------------------------------------------------------------------------------
+# B, Hq, Hkv, N, window, n_sink, d_qk, d_v, lens: blocks of sinks of 16 to 128 columns below the window, with P over the scores (d_v > 64) and beside
+SINKS = [(1, 4, 2, 700, 100, ns, d, dv, None) for ns in (17, 40, 64, 100, 130, 200) for d, dv in ((128, 128), (64, 128), (64, 64))] + [
+    (1, 3, 3, 900, 200, 70, 128, 128, [811]),
+    (1, 3, 3, 600, 100, 90, 128, 64, [555]),
+    (2, 2, 1, 400, 70, 9, 256, 256, [400, 288]),            # beyond the tensor-core kernels
+    (1, 2, 2, 300, 64, 33, 136, 40, None),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF], ids=["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("case", SINKS, ids=str)
+def test_blocks_of_sinks_of_every_width(case, dtype):
+    _, _, _, _, W, ns, _, _, lens = case
+    t, scale = attn_case(case, dtype)
+    want, bound = orc.attention(t["q"], t["k"], t["v"], lens, W, ns, scale, t["do"])
+    got = run_attn(t, lens_tensor(lens), W, ns, scale)
+    for n in want:
+        orc.check(got[n], want[n], bound[n], n)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan"), float("-inf")])
+@pytest.mark.parametrize("dtype", [F32, F16, BF], ids=["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("ns", [40, 130])
+@pytest.mark.parametrize("d, dv", [(128, 128), (64, 128), (128, 64)])
+def test_infinities_of_a_value_or_a_key(d, dv, ns, dtype, bad):
+    """One element of a value: o loses one column of the rows that see it, dV nothing at all.  One element of a key: a row whose score with it is
+    -inf goes on without it."""
+    N, W, j, c = 420, 100, 205, 3
+    t, scale = attn_case((1, 2, 1, N, W, ns, d, dv, None), dtype)
+    want, bound = orc.attention(t["q"], t["k"], t["v"], None, W, ns, scale, t["do"])
+    i = torch.arange(N)
+    sees = (i >= j) & (i < j + W)
+    inside = lambda got, n, at: bool(((got[n].double().cpu() - want[n]).abs() <= bound[n])[at].all())
+    planted = {n: x.clone() for n, x in t.items()}
+    planted["v"][0, 0, j, c] = bad
+    got = run_attn(planted, None, W, ns, scale)
+    others = torch.arange(dv) != c
+    assert not torch.isfinite(got["o"][0][:, sees, c]).any()
+    assert inside(got, "o", (0, slice(None), ~sees)) and inside(got, "o", (0, slice(None), slice(None), others))
+    assert inside(got, "lse", (0,)) and inside(got, "dv", (0,)) and inside(got, "dq", (0, slice(None), ~sees))
+    assert not torch.isfinite(got["dq"][0][:, sees]).all(-1).any()
+    alone = ((i - j).abs() >= W) & (i >= ns)                 # keys that no row sees together with j
+    assert inside(got, "dk", (0, slice(None), alone))
+    planted = {n: x.clone() for n, x in t.items()}
+    planted["k"][0, 0, j, c] = bad
+    o = run_attn(planted, None, W, ns, scale)["o"].double().cpu()
+    assert bool(((o - want["o"]).abs() <= bound["o"])[0][:, ~sees].all())
+    minus = sees & (t["q"][0, :, :, c].double() * bad == float("-inf"))
+    assert not torch.isfinite(o[0][sees & ~minus]).any()
+    if bad == bad:
+        # without key j: the same rows with a key that scores far below the others
+        low = {n: x.double() for n, x in t.items()}
+        see = orc.visible(N, W, ns, N)
+        see[:, j] = False
+        S = (low["q"][0] @ low["k"][0, 0].T * scale).masked_fill(~see, float("-inf"))
+        ref = torch.softmax(S, -1) @ low["v"][0, 0]
+        # (each weight is off by as much as in the row with key j, relative to itself)
+        off = (ref.abs() + torch.softmax(S, -1) @ low["v"][0, 0].abs()) * (2 * orc.HALF[dtype] + 2.0 ** -16) + orc.floor_of(dtype) * N
+        assert bool(((o[0] - ref).abs() <= off)[minus].all())
