@@ -301,12 +301,22 @@ cudaError_t launch_split_dims(const swa::sink::DecodeArgs& a, unsigned units, cu
 
 cudaError_t launch_split(int dtype, swa::sink::DecodeArgs& a, cudaStream_t st) {
   const unsigned units = (unsigned)a.B * a.Hkv * ((a.G + swa::sink::kDecHeads - 1) / swa::sink::kDecHeads);
-  // CTAs of a cluster: as many as fill the GPU's 296 places (two on an SM) once, while every warp keeps two tiles of 16 tokens.
-  // Measured (bf16, d = 128, us with 1 / 2 / 4 / 8 / 16): 8 pairs of sequence and key head, 2052 tokens 25 / 17 / 11.5 / 9.3 / 9.7; 64 pairs,
-  // 6004 tokens 104 / 62 / 41 / 48 / 73; 512 pairs, 4100 tokens 187 / 202 / 213 / 260 / 440.
+  // CTAs of a cluster: as many as there is room for at once, while every warp keeps two tiles of 16 tokens.  Clusters of up to 4 find two
+  // places on every SM; larger ones have to fit into a GPC: those of 8 gain while there is an SM for each CTA, those of 16 while each has a
+  // GPC, of which there are eight, of its own.  Measured (bf16, d = 128, us of a launch with 16 / 8 / 4 CTAs, cold L2):
+  //   pairs of sequence and key head     2052 tokens           6004 tokens
+  //                               4      14.3 / 14.3 / 17.6    16.4 / 20.5 / 28.0
+  //                               8      16.4 / 15.4 / 18.4    20.6 / 20.5 / 28.7      (launches in a row, 2052 tokens: 10.2 / 10.5)
+  //                               9      16.4 / 16.4 / 18.4    22.5 / 20.6 / 28.7
+  //                              12      17.6 / 16.4 / 18.4    23.8 / 22.5 / 28.7
+  //                              16      26.5 / 18.4 / 18.4    36.9 / 30.7 / 30.2
+  //                              24         - / 20.1 / 18.4       - / 34.8 / 33.0
+  //                              40         - / 30.7 / 26.6       - / 55.3 / 53.3
+  // and with 4 / 2 / 1: 64 pairs, 6004 tokens 41 / 62 / 104; 512 pairs, 4100 tokens 213 / 202 / 187.
   const int64_t seen = std::min((int64_t)a.W + a.ns, (int64_t)a.max_pages * a.page_size);
+  auto room = [](int c) { return c <= 4 ? 2 * 148 + 24 : c == 8 ? 148 : 8 * 16; };
   a.split = 1;
-  while (a.split < 16 && (int64_t)units * a.split * 2 <= 2 * 148 + 24 && seen > (int64_t)a.split * swa::sink::kDecWarps * 32) a.split *= 2;
+  while (a.split < 16 && (int64_t)units * a.split * 2 <= room(2 * a.split) && seen > (int64_t)a.split * swa::sink::kDecWarps * 32) a.split *= 2;
   a.page_shift = -1;
   if ((a.page_size & (a.page_size - 1)) == 0)
     for (a.page_shift = 0; 1 << a.page_shift < a.page_size;) ++a.page_shift;
