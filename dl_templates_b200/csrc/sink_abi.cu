@@ -210,7 +210,7 @@ int launch_rotate(swa::axes::Args& a, int n_groups, const swa_tensor_t* const* t
   }
   // Four heads a thread where that leaves two blocks for every place on the SMs (8 of 148): their loads are in flight together and the
   // table is read once (168 MB of bf16 rows: 32 us, one head a thread 41); fewer rows want the blocks (173 tokens: 2.1 us).
-  const bool four = a.N * spr / 256 * B * ((heads + 3) / 4) >= 2 * 8 * 148;
+  const bool four = a.N * spr / 256 * B * ((heads + 3) / 4) >= 2 * 8 * swa::sink::kSms;
   int64_t chunks = 0;
   for (int i = 0; i < n_groups; ++i) chunks += a.g[i].chunks = four ? (a.g[i].H + 3) / 4 : a.g[i].H;
   if (a.N * spr > INT32_MAX || a.N * spr * chunks > INT32_MAX) return fail(E_SHAPE, "too many tokens in one call");
@@ -314,7 +314,8 @@ cudaError_t launch_split(int dtype, swa::sink::DecodeArgs& a, cudaStream_t st) {
   //                              40         - / 30.7 / 26.6       - / 55.3 / 53.3
   // and with 4 / 2 / 1: 64 pairs, 6004 tokens 41 / 62 / 104; 512 pairs, 4100 tokens 213 / 202 / 187.
   const int64_t seen = std::min((int64_t)a.W + a.ns, (int64_t)a.max_pages * a.page_size);
-  auto room = [](int c) { return c <= 4 ? 2 * 148 + 24 : c == 8 ? 148 : 8 * 16; };
+  using swa::sink::kSms;
+  auto room = [](int c) { return c <= 4 ? 2 * kSms + 24 : c == 8 ? kSms : 8 * 16; };
   a.split = 1;
   while (a.split < 16 && (int64_t)units * a.split * 2 <= room(2 * a.split) && seen > (int64_t)a.split * swa::sink::kDecWarps * 32) a.split *= 2;
   a.page_shift = -1;

@@ -92,8 +92,9 @@ __global__ void __launch_bounds__(32 * kRowWarps) decode_rows_kernel(const __gri
 // the other warps -- and the partial results (maximum, sum, O) are joined once at the end, in the order of the warps, through
 // the shared memories of the cluster: one launch, no workspace, the same bits every time.
 // Bound by HBM: each visible key and value is read once for all heads of its group.  With 16-bit types both products are warp MMAs with
-// the heads as columns, S^T = K Q^T (16 keys x 8 heads) and O^T += V^T P^T: with the heads as 16 rows a tile took 627 instructions and 64
-// accumulators a thread, most of them for heads that are not there.  fp32 runs on the CUDA cores, lanes by keys for the scores and by columns for O.
+// the heads as columns, S^T = K Q^T (16 keys x 8 heads) and O^T += V^T P^T, P rounded to the type of V as in the forward kernel: with the heads
+// as 16 rows a tile took 627 instructions and 64 accumulators a thread, most of them for heads that are not there.  fp32 runs on the CUDA
+// cores, lanes by keys for the scores and by columns for O.
 // The weights are taken at the running maximum, so that no tile waits for a reduction over its lanes (64 sequences, 4100 tokens, 32 heads of
 // 128 on 8, bf16: 186 us, 5.8 TB/s of 6.5 measured for a copy; one sequence of 2052 tokens 9.7 us, most of it the chain length -> page ->
 // data -> join).  fp32: 16 sequences of 2004 tokens 81 us, 3.2 TB/s, bound by the multiply-adds' shared memory reads.

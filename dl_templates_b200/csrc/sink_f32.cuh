@@ -34,7 +34,7 @@ constexpr int kF32Y = kF32Threads / 16;           // rows ty + kF32Y i of a thre
 struct F32Params {
   Args a;
   int n_t, n_sb, pieces, piece_len, near, n_sink_items;   // KIND 2: blocks that hold sinks, their pieces (cut_pieces)
-  float* part;                                      // [B, Hkv, n_sb, pieces, 64, d_qk + d_v]
+  float* part;                                      // [B, Hkv, n_sb, pieces, kF32X, d_qk + d_v]
 };
 
 template <int KIND, int DQ, int DV>
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kF32Threads, (KIND == 2 && DQ + DV > 128 ? 1 :
   const Args& a = p.a;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
 
-  // ---- the item: resident rows x0 .. x0 + 63 of head h, the blocks it streams
+  // ---- the item: resident rows x0 .. x0 + kF32X - 1 of head h, the blocks it streams
   int b, h, x0, piece = -1, nb, first = 0, per_head = 0, hi = 0, lo = 0, sb = 0;
   if constexpr (KIND != 2) {
     const int per = a.B * a.Hq, r = blockIdx.x % per;

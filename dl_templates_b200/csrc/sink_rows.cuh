@@ -12,6 +12,9 @@
 namespace swa {
 namespace sink {
 
+// SMs of a B200.  The rules that cut work take this number and do not ask the device: the cut decides in which order sums are made, so that a
+// part of a GPU gives the same bits.
+constexpr int kSms = 148;
 constexpr int kMaxDim = 256, kDimsPerLane = kMaxDim / 32;
 
 struct Args {
@@ -304,7 +307,7 @@ inline Pieces cut_pieces(const Args& a, int n_sb, int rows, int stream) {
   Pieces c;
   c.near = (rows - 1 + a.W + stream - 1) / stream;
   const int64_t all = (int64_t)a.G * ((a.N + stream - 1) / stream), blocks = (int64_t)a.B * a.Hkv * n_sb;
-  const int64_t busy = (4 * 148 + blocks - 1) / (blocks > 0 ? blocks : 1), patient = ((int64_t)a.G * a.N >> 24) + 1;
+  const int64_t busy = (4 * kSms + blocks - 1) / (blocks > 0 ? blocks : 1), patient = ((int64_t)a.G * a.N >> 24) + 1;
   const int64_t cap = busy > patient ? busy : patient, shortest = (all + cap - 1) / cap, ordinary = (int64_t)a.G * c.near;
   const int64_t len = ordinary > shortest ? ordinary : shortest;
   c.len = (int)(len < INT32_MAX ? len : INT32_MAX);

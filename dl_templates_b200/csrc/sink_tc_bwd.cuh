@@ -18,13 +18,16 @@
 // waited for.  The scores of the next block are made while a block's P and dS are, its dP as soon as
 // this block's has been read, and this block's products run behind it.
 //
-// Measured (bf16, 16384 tokens, window 1024, 64 sinks, 16 heads of 128 on 4): dQ 236 us, tensor pipe 56 % busy; dK/dV 293 us, 67 %; with what the
-// kernels execute, 7 products and whole blocks, that is 1.05 PFLOP/s.  Left: per block about 200 cycles of waits, 860 for 48 columns of P,
+// Measured (bf16, 16384 tokens, window 1024, 64 sinks, 16 heads of 128 on 4): dQ 217 to 236 us, tensor pipe 56 % busy; dK/dV 266 to 293 us, 67 %; with what the
+// kernels execute, 7 products and whole blocks, that is 1.05 to 1.15 PFLOP/s.  Left: per block about 200 cycles of waits, 860 for 48 columns of P,
 // 380 for dS, 350 of loop.  Tried and not kept: the groups on alternate whole blocks with a dP buffer each, which wants N = 96 and 64 (dQ 222 us,
 // dK/dV 291; with heads of 64 dQ 91 -> 109 and dK/dV 119 -> 132).
 //
 // Blocks of dK/dV that hold sinks are seen by every later query: their stream is cut into pieces about as long as another block's, the
 // partial sums go to scratch in fp32 and join_kernel (sink_rows.cuh) adds them in order.
+//
+// P and dS are rounded to the type of the tensors they are multiplied with, as in the forward kernel; delta is made from the rounded O.  Error
+// against 64 bits, as multiples of the results' own rounding: dV 1.4, dQ and dK 1.46 to 1.53 (1.05 to 1.1 with P and dS in fp32: what delta adds).
 //
 // Infinities and NaN: as in the forward kernel, rows of the result that end as one are done again by row_dq / row_dkdv, rows of a piece's
 // sums by row_piece; padding behind a sequence's end is zeros before it is multiplied.

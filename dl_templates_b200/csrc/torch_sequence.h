@@ -163,8 +163,6 @@ std::array<Tensor, 2> rotate_axes(const Tensor& x, const Tensor& x2, Axes ax, bo
 struct AxesNode : public torch::autograd::Node {
   SavedVariable pos;
   std::vector<SavedVariable> tables;
-  std::array<std::vector<int64_t>, 2> sizes;
-  at::TensorOptions options;
 
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
